@@ -10,7 +10,7 @@ The native library (libgloo_amd.so, C ABI in include/gloo_amd/glx.h) is
 required; there is no CPU fallback.
 """
 from . import _lib  # noqa: F401  (raises ImportError if the HIP build is missing)
-from . import math, rendezvous  # noqa: F401
+from . import math, mx, rendezvous  # noqa: F401
 from .algorithms import (  # noqa: F401
     AllreduceBcube,
     AllreduceHalvingDoubling,
@@ -32,6 +32,7 @@ from .algorithms import (  # noqa: F401
 )
 from .collectives import AllreduceOptions, allreduce  # noqa: F401
 from .events import Event  # noqa: F401
+from .gradients import Gradients  # noqa: F401
 from . import errors  # noqa: F401
 from .errors import EnforceNotMet, Exception, HipError, IoException  # noqa: F401,A004
 

@@ -27,7 +27,7 @@ if not os.path.exists(LIB_PATH):
 lib = ctypes.CDLL(LIB_PATH)
 
 _vp, _sz, _i, _i64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_int64
-_pi = ctypes.POINTER(ctypes.c_int)
+_pi, _d = ctypes.POINTER(ctypes.c_int), ctypes.c_double
 
 # (name, restype, argtypes) for every symbol declared in include/gloo_amd/glx.h
 SIGNATURES = [
@@ -124,6 +124,18 @@ SIGNATURES = [
     ("glx_set_engine_streams", _i, [_i]),
     ("glx_allreduce", _i, [_vp, _i, _i, _i, ctypes.POINTER(_vp), _i, ctypes.POINTER(_vp), _i,
                            ctypes.c_size_t, ctypes.c_uint32, ctypes.c_size_t, _i64, _vp]),
+    ("glx_gradients_create", _vp, [ctypes.POINTER(_vp), ctypes.POINTER(_vp), ctypes.POINTER(_sz),
+                                   _pi, _i]),
+    ("glx_gradients_destroy", None, [_vp]),
+    ("glx_gradients_device", _i, [_vp]),
+    ("glx_gradients_workspace_bytes", _sz, [_vp]),
+    ("glx_gradients_power_sum", _i, [_vp, _d, _vp, _vp, _vp]),
+    ("glx_gradients_norm", _i, [_vp, _d, _vp, _i, _vp, _vp]),
+    ("glx_gradients_clip", _i, [_vp, _d, _d, _vp, _vp, _i, _vp, _vp]),
+    ("glx_mx_payload_bytes", _sz, [_sz]),
+    ("glx_mx_quantize", _i, [_i, _vp, _vp, _vp, _vp, _sz, _vp]),
+    ("glx_mx_reduce_n", _i, [_i, _vp, ctypes.POINTER(_vp), _i, _sz, ctypes.c_float, _vp]),
+    ("glx_mx_requantize_n", _i, [_vp, ctypes.POINTER(_vp), _i, _sz, ctypes.c_float, _vp]),
 ]
 
 for _name, _res, _args in SIGNATURES:

@@ -3,6 +3,7 @@
 // returns a GLX_ERR_* code; nothing throws across the ABI.
 #include <hip/hip_runtime_api.h>
 
+#include <cmath>
 #include <cstring>
 #include <memory>
 #include <string>
@@ -13,10 +14,12 @@
 #include "context.h"
 #include "executor.h"
 #include "executor_internal.h"
+#include "gradients.h"
 #include "host_fn.h"
 #include "host_ops.h"
 #include "kernels.h"
 #include "linkprobe.h"
+#include "mx.h"
 #include "plan.h"
 #include "store.h"
 
@@ -37,6 +40,9 @@ struct glx_algorithm {
 };
 struct glx_link_probe {
   std::unique_ptr<gloo::LinkProbe> p;
+};
+struct glx_gradients {
+  std::unique_ptr<gloo::GradientList> g;
 };
 
 namespace {
@@ -108,6 +114,23 @@ glx::PlanParams planParams(int esize, int64_t maxSegmentBytes, int64_t minPieceB
   // glx_set_pipeline_bytes (the CPU tests replay them)
   p.pipelineBytes = glx::pipelineBytes();
   return p;
+}
+
+bool mxDtype(int d) { return d == GLX_FLOAT32 || d == GLX_FLOAT16 || d == GLX_BFLOAT16; }
+
+// Whether [a, a + na) and [b, b + nb) share a byte.
+bool overlaps(const void* a, size_t na, const void* b, size_t nb) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return a != nullptr && b != nullptr && x < y + nb && y < x + na;
+}
+
+void checkMxPayloads(const void* const* payloads, int k) {
+  GLX_ENFORCE(payloads != nullptr && k >= 1 && k <= glx::kMxMaxSources,
+              "mx: need 1..", glx::kMxMaxSources, " payloads");
+  for (int j = 0; j < k; j++) {
+    GLX_ENFORCE(payloads[j] != nullptr && (uintptr_t)payloads[j] % 16 == 0, "mx: payload ", j,
+                " is null or not 16-byte aligned");
+  }
 }
 
 }  // namespace
@@ -975,6 +998,135 @@ int64_t glx_plan_fold_ex(int algo, int rank, int size, int64_t count, int esize,
     return GLX_OK;
   });
   return n;
+}
+
+// ---- gradients --------------------------------------------------------------
+
+glx_gradients* glx_gradients_create(void* const* grads, void* const* outs,
+                                    const size_t* counts, const int* dtypes, int n) {
+  glx_gradients* out = nullptr;
+  guarded([&]() -> int {
+    GLX_ENFORCE(n >= 0, "glx_gradients_create: negative number of tensors");
+    GLX_ENFORCE(n == 0 || (grads != nullptr && counts != nullptr && dtypes != nullptr),
+                "glx_gradients_create: null array");
+    std::vector<void*> g(grads, grads + n), o;
+    if (outs != nullptr) o.assign(outs, outs + n);
+    std::unique_ptr<gloo::GradientList> list(
+        new gloo::GradientList(g, o, std::vector<size_t>(counts, counts + n),
+                               std::vector<int>(dtypes, dtypes + n)));
+    out = new glx_gradients{std::move(list)};
+    return GLX_OK;
+  });
+  return out;
+}
+
+void glx_gradients_destroy(glx_gradients* g) { delete g; }
+
+int glx_gradients_device(const glx_gradients* g) { return g == nullptr ? -1 : g->g->device(); }
+
+size_t glx_gradients_workspace_bytes(const glx_gradients* g) {
+  return g == nullptr ? 0 : g->g->workspaceBytes();
+}
+
+int glx_gradients_power_sum(const glx_gradients* g, double p, void* sum, void* workspace,
+                            glx_stream_t stream) {
+  return guarded([&]() -> int {
+    GLX_ENFORCE(g != nullptr, "glx_gradients_power_sum: null handle");
+    g->g->powerSum(p, sum, workspace, (hipStream_t)stream);
+    return GLX_OK;
+  });
+}
+
+int glx_gradients_norm(const glx_gradients* g, double p, void* norm, int norm_dtype,
+                       void* workspace, glx_stream_t stream) {
+  return guarded([&]() -> int {
+    GLX_ENFORCE(g != nullptr, "glx_gradients_norm: null handle");
+    g->g->norm(p, norm, norm_dtype, workspace, (hipStream_t)stream);
+    return GLX_OK;
+  });
+}
+
+int glx_gradients_clip(const glx_gradients* g, double max_norm, double p,
+                       const void* power_sum, void* norm, int norm_dtype, void* workspace,
+                       glx_stream_t stream) {
+  return guarded([&]() -> int {
+    GLX_ENFORCE(g != nullptr, "glx_gradients_clip: null handle");
+    g->g->clip(max_norm, p, power_sum, norm, norm_dtype, workspace, (hipStream_t)stream);
+    return GLX_OK;
+  });
+}
+
+// ---- microscaled messages ---------------------------------------------------
+
+size_t glx_mx_payload_bytes(size_t n) { return glx::mxPayloadBytes(n); }
+
+int glx_mx_quantize(int dtype, void* payload, const void* x, const float* residual,
+                    float* residual_out, size_t n, glx_stream_t stream) {
+  return guarded([&]() -> int {
+    GLX_ENFORCE(mxDtype(dtype), "glx_mx_quantize: float32, float16 or bfloat16");
+    GLX_ENFORCE(n <= (size_t(1) << 60), "glx_mx_quantize: too many elements");
+    if (n == 0) return GLX_OK;
+    const size_t es = glx_dtype_size(dtype), bytes = glx::mxPayloadBytes(n);
+    checkMxPayloads(&payload, 1);
+    GLX_ENFORCE(x != nullptr && (uintptr_t)x % es == 0, "glx_mx_quantize: null or misaligned x");
+    GLX_ENFORCE((uintptr_t)residual % 4 == 0 && (uintptr_t)residual_out % 4 == 0,
+                "glx_mx_quantize: misaligned residual");
+    GLX_ENFORCE(!overlaps(payload, bytes, x, n * es) &&
+                    !overlaps(payload, bytes, residual, n * 4) &&
+                    !overlaps(payload, bytes, residual_out, n * 4),
+                "glx_mx_quantize: the payload shares memory with another buffer");
+    GLX_ENFORCE(residual_out == residual || !overlaps(residual_out, n * 4, residual, n * 4),
+                "glx_mx_quantize: the residuals overlap");
+    GLX_ENFORCE((const void*)residual_out == x ? dtype == GLX_FLOAT32
+                                               : !overlaps(residual_out, n * 4, x, n * es),
+                "glx_mx_quantize: residual_out overlaps x");
+    gloo::DeviceScope scope(gloo::deviceOf(payload));
+    return hipStatus(glx::launch_mx_quantize(dtype, payload, x, residual, residual_out, n,
+                                             (hipStream_t)stream),
+                     "glx_mx_quantize");
+  });
+}
+
+int glx_mx_reduce_n(int dtype, void* dst, const void* const* payloads, int k, size_t n,
+                    float scale, glx_stream_t stream) {
+  return guarded([&]() -> int {
+    GLX_ENFORCE(mxDtype(dtype), "glx_mx_reduce_n: float32, float16 or bfloat16");
+    GLX_ENFORCE(n <= (size_t(1) << 60), "glx_mx_reduce_n: too many elements");
+    GLX_ENFORCE(std::isfinite(scale), "glx_mx_reduce_n: scale is not finite");
+    if (n == 0) return GLX_OK;
+    const size_t es = glx_dtype_size(dtype), bytes = glx::mxPayloadBytes(n);
+    checkMxPayloads(payloads, k);
+    GLX_ENFORCE(dst != nullptr && (uintptr_t)dst % es == 0,
+                "glx_mx_reduce_n: null or misaligned dst");
+    for (int j = 0; j < k; j++) {
+      GLX_ENFORCE(!overlaps(dst, n * es, payloads[j], bytes), "glx_mx_reduce_n: dst and payload ",
+                  j, " share memory");
+    }
+    gloo::DeviceScope scope(gloo::deviceOf(dst));
+    return hipStatus(
+        glx::launch_mx_reduce_n(dtype, dst, payloads, k, n, scale, (hipStream_t)stream),
+        "glx_mx_reduce_n");
+  });
+}
+
+int glx_mx_requantize_n(void* payload, const void* const* payloads, int k, size_t n,
+                        float scale, glx_stream_t stream) {
+  return guarded([&]() -> int {
+    GLX_ENFORCE(n <= (size_t(1) << 60), "glx_mx_requantize_n: too many elements");
+    GLX_ENFORCE(std::isfinite(scale), "glx_mx_requantize_n: scale is not finite");
+    if (n == 0) return GLX_OK;
+    const size_t bytes = glx::mxPayloadBytes(n);
+    checkMxPayloads(payloads, k);
+    checkMxPayloads(&payload, 1);
+    for (int j = 0; j < k; j++) {
+      GLX_ENFORCE(payload == payloads[j] || !overlaps(payload, bytes, payloads[j], bytes),
+                  "glx_mx_requantize_n: the payload overlaps source ", j);
+    }
+    gloo::DeviceScope scope(gloo::deviceOf(payload));
+    return hipStatus(
+        glx::launch_mx_requantize_n(payload, payloads, k, n, scale, (hipStream_t)stream),
+        "glx_mx_requantize_n");
+  });
 }
 
 }  // extern "C"

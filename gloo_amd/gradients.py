@@ -1,0 +1,148 @@
+"""The global norm of a list of gradients, and clipping by it: what a
+data-parallel program does with the buffers its allreduce returns.
+
+    g = gloo_amd.Gradients(grads)          # the tensors' memory, laid out once
+    total = g.clip_norm(1.0)               # in place; the norm, on the device
+"""
+import ctypes
+
+from . import _lib
+from .algorithms import FLOAT32, FLOAT64, _stream_ptr, torch_dtype_code
+from .errors import check, check_handle
+
+lib = _lib.lib
+
+
+def _dense(t):
+    """Whether the elements of t fill one stretch of memory, in any order."""
+    expect = 1
+    for stride, size in sorted(zip(t.stride(), t.shape)):
+        if size == 1:
+            continue
+        if stride != expect:
+            return False
+        expect *= size
+    return True
+
+
+class Gradients:
+    """Gradient tensors of one device (float32, float64, float16 or bfloat16,
+    mixed as they come; empty ones too).  A tensor may start at any element of
+    its storage and have its dimensions in any order, but its elements fill
+    one stretch of memory.  With `outs`, tensors of the same types, shapes and
+    strides, clip_norm writes there and leaves the gradients as they are
+    (outs[i] may be grads[i]).  Tensors that share memory are refused.
+
+    The object keeps the memory that the tensors have when it is made, as the
+    allreduce classes do: after giving a parameter another gradient tensor,
+    make another one.  Calls enqueue on `stream` (torch.cuda.Stream or raw
+    hipStream_t; default: torch's current stream) without synchronising, and
+    can be captured in a HIP graph; each has a workspace of its own, so they
+    may run at once on several streams.  The caller orders them after whatever
+    wrote the gradients, and keeps the object alive while its work, or a graph
+    holding it, runs."""
+
+    def __init__(self, grads, outs=None):
+        import torch
+        grads = list(grads)
+        outs = None if outs is None else list(outs)
+        if outs is not None and len(outs) != len(grads):
+            raise ValueError("%d gradients, %d outs" % (len(grads), len(outs)))
+        self._h = None
+        codes = []
+        for i, t in enumerate(grads):
+            code = torch_dtype_code(t)
+            if not t.dtype.is_floating_point:
+                raise TypeError("gradient %d is %s" % (i, t.dtype))
+            codes.append(code)
+            if not t.is_cuda or t.device != grads[0].device:
+                raise ValueError("gradient %d is on %s" % (i, t.device))
+            if t.numel() and not _dense(t):
+                raise ValueError("gradient %d has gaps or overlaps in its memory (strides %s)"
+                                 % (i, tuple(t.stride())))
+            if outs is None:
+                continue
+            o = outs[i]
+            if o.dtype != t.dtype:
+                raise TypeError("out %d is %s, its gradient %s" % (i, o.dtype, t.dtype))
+            if o.device != t.device or o.shape != t.shape or (
+                    t.numel() and any(a != b for a, b, s in zip(o.stride(), t.stride(), t.shape)
+                                      if s > 1)):
+                raise ValueError("out %d does not have its gradient's device, shape and strides"
+                                 % i)
+        n = len(grads)
+        self.device = grads[0].device if grads else torch.device(
+            "cuda", torch.cuda.current_device())
+        self.dtype = torch.float64 if any(t.dtype == torch.float64 for t in grads) \
+            else torch.float32  # of the norm
+        self._code = FLOAT64 if self.dtype == torch.float64 else FLOAT32
+        # aliases hold the memory, also if a tensor is given another later
+        self._keep = [t.detach() for t in grads] + [t.detach() for t in outs or ()]
+        ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in grads])
+        optr = None if outs is None else (ctypes.c_void_p * n)(*[t.data_ptr() for t in outs])
+        self._h = check_handle(
+            lib.glx_gradients_create(ptrs, optr, (ctypes.c_size_t * n)(*[t.numel() for t in grads]),
+                                     (ctypes.c_int * n)(*codes), n), "Gradients")
+        self._ws = lib.glx_gradients_workspace_bytes(self._h) // 8
+
+    def _scalar(self, t, dtype, what):
+        if t.dtype != dtype or t.numel() != 1 or t.device != self.device:
+            raise ValueError("%s: one %s on %s" % (what, dtype, self.device))
+        return t.data_ptr()
+
+    def _call(self, fn, dtype, out, stream, args):
+        """fn(handle, *args(out pointer, workspace pointer), stream)."""
+        import torch
+        if self._h is None:
+            raise ValueError("Gradients: closed")
+        if stream is None:
+            stream = torch.cuda.current_stream(self.device)
+        elif stream != torch.cuda.current_stream(self.device):
+            # what is allocated here belongs to the stream that uses it
+            own = torch.cuda.ExternalStream(stream, self.device) if isinstance(stream, int) \
+                else stream
+            with torch.cuda.stream(own):
+                return self._call(fn, dtype, out, None, args)
+        if out is None:
+            out = torch.empty((), dtype=dtype, device=self.device)
+        else:
+            self._scalar(out, dtype, "out")
+        ws = torch.empty(self._ws, dtype=torch.float64, device=self.device)
+        check(fn(self._h, *args(out.data_ptr(), ws.data_ptr()), _stream_ptr(stream)),
+              "Gradients")
+        return out
+
+    def power_sum(self, p=2.0, out=None, stream=None):
+        """The sum of |x|^p over all gradients (the maximum of |x| for
+        p = inf; p is 1, 2 or inf), accumulated in and returned as float64.
+        Ranks holding shards allreduce it (SUM; MAX for inf) and give it to
+        clip_norm."""
+        import torch
+        return self._call(lib.glx_gradients_power_sum, torch.float64, out, stream,
+                          lambda o, ws: (float(p), o, ws))
+
+    def norm(self, p=2.0, out=None, stream=None):
+        """The p-norm of all gradients together: float32, or float64 if one
+        of them is."""
+        return self._call(lib.glx_gradients_norm, self.dtype, out, stream,
+                          lambda o, ws: (float(p), o, self._code, ws))
+
+    def clip_norm(self, max_norm, p=2.0, power_sum=None, out=None, stream=None):
+        """Scale every gradient by min(1, max_norm / (norm + 1e-6)), in place
+        or into outs, and return the norm (as norm() does): the list's own,
+        or that of power_sum (a float64 on the device).  A NaN norm makes
+        every gradient NaN, an infinite one 0 (NaN where it was infinite)."""
+        import torch
+        total = None if power_sum is None else self._scalar(power_sum, torch.float64, "power_sum")
+        return self._call(lib.glx_gradients_clip, self.dtype, out, stream,
+                          lambda o, ws: (float(max_norm), float(p), total, o,
+                                         self._code, ws))
+
+    def close(self):
+        """Free the handle (its work, and graphs holding it, must be done)."""
+        h, self._h = getattr(self, "_h", None), None
+        if h:
+            lib.glx_gradients_destroy(h)
+
+    def __del__(self):
+        self.close()

@@ -744,4 +744,96 @@ inline void allreduce(const AllreduceOptions& opts) {
         "allreduce");
 }
 
+// The global norm of a list of gradients on one device, and clipping by it
+// (glx_gradients_*): laid out once, as the algorithms take their pointers.
+//   Gradients g(Gradients::List().add(p0, n0).add(p1, n1));
+//   g.clipNorm(1.0f, norm, workspace, stream);
+// Scalars and workspaces (workspaceBytes()) are device memory; calls enqueue
+// and never synchronise.
+class Gradients {
+ public:
+  // Tensors in order; `out` (default: in place) receives the clipped values.
+  class List {
+   public:
+    template <typename T>
+    List& add(T* grad, size_t count, T* out = nullptr) {
+      grads_.push_back(grad);
+      outs_.push_back(out == nullptr ? grad : out);
+      counts_.push_back(count);
+      dtypes_.push_back(DType<T>::value);
+      return *this;
+    }
+
+   private:
+    std::vector<void*> grads_, outs_;
+    std::vector<size_t> counts_;
+    std::vector<int> dtypes_;
+    friend class Gradients;
+  };
+
+  explicit Gradients(const List& l)
+      : g_(checkHandle(glx_gradients_create(l.grads_.data(), l.outs_.data(), l.counts_.data(),
+                                            l.dtypes_.data(), (int)l.grads_.size()),
+                       "Gradients")) {}
+  ~Gradients() { glx_gradients_destroy(g_); }
+  Gradients(const Gradients&) = delete;
+  Gradients& operator=(const Gradients&) = delete;
+
+  int device() const { return glx_gradients_device(g_); }
+  size_t workspaceBytes() const { return glx_gradients_workspace_bytes(g_); }
+  void powerSum(double p, double* sum, void* workspace, glx_stream_t stream) const {
+    check(glx_gradients_power_sum(g_, p, sum, workspace, stream), "Gradients::powerSum");
+  }
+  // F: float or double
+  template <typename F>
+  void norm(double p, F* norm, void* workspace, glx_stream_t stream) const {
+    check(glx_gradients_norm(g_, p, norm, DType<F>::value, workspace, stream),
+          "Gradients::norm");
+  }
+  template <typename F>
+  void clipNorm(double maxNorm, F* norm, void* workspace, glx_stream_t stream,
+                double p = 2) const {
+    check(glx_gradients_clip(g_, maxNorm, p, nullptr, norm, DType<F>::value, workspace, stream),
+          "Gradients::clipNorm");
+  }
+  // by the allreduced power sum of all ranks' shards
+  template <typename F>
+  void clipNormOf(const double* powerSum, double maxNorm, F* norm, glx_stream_t stream,
+                  double p = 2) const {
+    check(glx_gradients_clip(g_, maxNorm, p, powerSum, norm, DType<F>::value, nullptr, stream),
+          "Gradients::clipNormOf");
+  }
+
+ private:
+  glx_gradients* g_;
+};
+
+// Microscaled 4-bit messages (glx_mx_*).  T: float, float16 or bfloat16.
+namespace mx {
+
+inline size_t payloadBytes(size_t n) { return glx_mx_payload_bytes(n); }
+
+template <typename T>
+void quantize(void* payload, const T* x, size_t n, glx_stream_t stream,
+              const float* residual = nullptr, float* residualOut = nullptr) {
+  check(glx_mx_quantize(DType<T>::value, payload, x, residual, residualOut, n, stream),
+        "mx::quantize");
+}
+
+template <typename T>
+void reduceN(T* dst, const std::vector<const void*>& payloads, size_t n, glx_stream_t stream,
+             float scale = 1) {
+  check(glx_mx_reduce_n(DType<T>::value, dst, payloads.data(), (int)payloads.size(), n, scale,
+                        stream),
+        "mx::reduceN");
+}
+
+inline void requantizeN(void* payload, const std::vector<const void*>& payloads, size_t n,
+                        glx_stream_t stream, float scale = 1) {
+  check(glx_mx_requantize_n(payload, payloads.data(), (int)payloads.size(), n, scale, stream),
+        "mx::requantizeN");
+}
+
+}  // namespace mx
+
 }  // namespace gloo_amd

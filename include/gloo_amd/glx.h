@@ -670,6 +670,83 @@ int64_t glx_plan_stage(int algo, int rank, int size, int64_t count, int esize,
                        int64_t max_piece, int64_t* h2d, int64_t h2d_cap, int64_t* d2h,
                        int64_t d2h_cap, int64_t* n_d2h);
 
+/* ---- gradients: global norm and clipping ------------------------------- */
+
+/* No reference counterpart: what a data-parallel program does with its
+ * gradients after the allreduce.  A handle lays a list of n tensors on one
+ * device out once, as the allreduce algorithms take their pointers: tensor i
+ * has counts[i] elements of dtypes[i] (FLOAT32, FLOAT64, FLOAT16 or BFLOAT16)
+ * at grads[i], contiguous and aligned to its elements only.  outs[i] receives
+ * its clipped values (outs NULL: in place).  Empty tensors are allowed, and an
+ * empty list.  Tensors that share memory are refused (a gradient listed twice
+ * would be scaled twice); outs[i] may be grads[i] but overlap nothing else.
+ * NULL on failure.  The memory must stay valid while the handle is used.
+ *
+ * The calls below enqueue on `stream` and never synchronise; they can be
+ * captured.  The handle is read-only after its creation, so calls on several
+ * streams, or captured graphs, may run at once if each has a workspace (device
+ * memory, glx_gradients_workspace_bytes, 8-byte aligned) of its own.  Destroy
+ * the handle after the work (and graphs) using it.
+ *
+ * p is 1, 2 or INFINITY: S = sum |x|^p over all tensors (the maximum for
+ * INFINITY), accumulated in float64, in an order that depends on the list
+ * alone; the norm is S^(1/p).  A NaN anywhere makes both NaN. */
+typedef struct glx_gradients glx_gradients;
+glx_gradients* glx_gradients_create(void* const* grads, void* const* outs,
+                                    const size_t* counts, const int* dtypes, int n);
+void glx_gradients_destroy(glx_gradients* g);
+/* Device index of the tensors, -1 for NULL. */
+int glx_gradients_device(const glx_gradients* g);
+size_t glx_gradients_workspace_bytes(const glx_gradients* g);
+/* *sum = S, a float64 in device memory.  Ranks that hold shards of the
+ * gradients allreduce it (SUM, or MAX for INFINITY) and hand it to
+ * glx_gradients_clip. */
+int glx_gradients_power_sum(const glx_gradients* g, double p, void* sum, void* workspace,
+                            glx_stream_t stream);
+/* *norm = S^(1/p), a float32 or float64 (norm_dtype) in device memory. */
+int glx_gradients_norm(const glx_gradients* g, double p, void* norm, int norm_dtype,
+                       void* workspace, glx_stream_t stream);
+/* outs[i] = grads[i] * min(1, max_norm / (norm + 1e-6)): the product in float32
+ * (float64 for FLOAT64 tensors), rounded once to the tensor's type.  The norm
+ * is the list's own, or that of power_sum (a float64 in device memory; the
+ * workspace is then not used and may be NULL), and is written to `norm` unless
+ * that is NULL.  A norm of NaN makes every output NaN, an infinite one makes
+ * them 0 (NaN where the gradient is infinite).  In place, tensors are not
+ * touched when the coefficient is 1. */
+int glx_gradients_clip(const glx_gradients* g, double max_norm, double p,
+                       const void* power_sum, void* norm, int norm_dtype, void* workspace,
+                       glx_stream_t stream);
+
+/* ---- microscaled 4-bit messages (OCP MX v1.0, MXFP4) -------------------- */
+
+/* No reference counterpart: 17/32 byte per element on the wire.  A payload of
+ * n elements (device memory, 16-byte aligned): nb = ceil(n / 32) blocks of 16
+ * bytes -- 32 E2M1 codes, two to a byte, the even element in the low half --,
+ * then nb scale bytes (E8M0: 2^(byte - 127); 255: every value of the block is
+ * NaN), then zero bytes up to a multiple of 16.  Codes behind element n - 1
+ * are 0.  Every byte of the payload is determined by the values. */
+size_t glx_mx_payload_bytes(size_t n);
+/* payload = the blocks of y = x + residual (in float32; residual NULL: y = x).
+ * A block's scale is that of its largest magnitude's power of two over 4 (the
+ * scale byte at least 0); codes are rounded to nearest even and saturate at
+ * 6.  A block holding an infinity or NaN becomes a NaN block.  residual_out
+ * (unless NULL) = y - what the payload stands for, exact in float32, and 0 in
+ * NaN blocks: the error to add to the next message.  dtype of x: FLOAT32,
+ * FLOAT16, BFLOAT16.  residual_out may be residual, or a FLOAT32 x; no other
+ * memory may be shared with what is written. */
+int glx_mx_quantize(int dtype, void* payload, const void* x, const float* residual,
+                    float* residual_out, size_t n, glx_stream_t stream);
+/* dst = scale * (v_0 + v_1 + ... + v_{k-1}): the left fold of the payloads'
+ * values in float32 (glx_reduce_n's order), times scale (finite) in float32,
+ * rounded once to dtype (FLOAT32, FLOAT16, BFLOAT16).  1 <= k <= 16; k = 1 with
+ * scale 1 opens one payload. */
+int glx_mx_reduce_n(int dtype, void* dst, const void* const* payloads, int k, size_t n,
+                    float scale, glx_stream_t stream);
+/* The same fold, its float32 result quantised again: one hop of a compressed
+ * exchange.  payload may be one of the sources. */
+int glx_mx_requantize_n(void* payload, const void* const* payloads, int k, size_t n,
+                        float scale, glx_stream_t stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif
