@@ -10,6 +10,13 @@ namespace gloo {
 
 namespace {
 
+// Lists of up to 64 chunks of 4 KiB are summed by one workgroup (64 chunks of f32:
+// 4.2 us, two launches 6.1), but only half as many are also clipped by it: the
+// CU that does it alone needs 6.1 us for 32 chunks and 7.7 for 64, of 16-bit
+// values 9.1, two launches 6.4 for any of them.
+constexpr int kShortClipChunks = 32;
+constexpr size_t kCachedBytes = size_t(256) << 20;  // the Infinity Cache
+
 size_t elementSize(int dtype) {
   switch (dtype) {
     case GLX_FLOAT64: return 8;
@@ -104,22 +111,28 @@ GradientList::GradientList(const std::vector<void*>& grads, const std::vector<vo
   int cus = 0;
   GLX_HIP_CHECK(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device_));
 
-  // Chunks of 64 KiB, shorter for lists too small to give every workgroup one.
-  const size_t groups = (size_t)std::max(cus, 1) * 8;
-  const size_t chunk =
-      std::min<size_t>(64 << 10, std::max<size_t>(4 << 10, bytes / groups / 4096 * 4096));
+  // Chunks of 16 KiB, one pass of a workgroup's loads, cut at 16-byte boundaries
+  // of the gradient; shorter where that would leave workgroups without one.
+  const size_t groups = (size_t)std::max(cus, 1) * 4;
+  const size_t chunk = std::min<size_t>(
+      16 << 10, std::max(glx::kGradShortBytes, bytes / groups / 4096 * 4096));
   std::vector<glx::GradChunk> table;
   for (size_t i = 0; i < grads.size(); i++) {
     const size_t es = elementSize(dtypes[i]), per = chunk / es;
     char* g = (char*)grads[i];
     char* o = outs.empty() ? g : (char*)outs[i];
-    for (size_t at = 0; at < counts[i]; at += per) {
-      table.push_back({g + at * es, o + at * es, (uint32_t)std::min(per, counts[i] - at),
-                       (uint32_t)dtypes[i]});
+    const size_t lead = (uintptr_t)g % 16 / es;
+    for (size_t at = 0, n; at < counts[i]; at += n) {
+      n = std::min(at == 0 ? per - lead : per, counts[i] - at);
+      table.push_back({g + at * es, o + at * es, (uint32_t)n, (uint32_t)dtypes[i]});
     }
   }
-  GLX_ENFORCE(table.size() < (size_t(1) << 31), "gradients: the list is too long");
+  // one workgroup of 256 threads per chunk, below 2^32 threads
+  GLX_ENFORCE(table.size() < (size_t(1) << 24) - 8, "gradients: the list is too long");
   nchunks_ = (int)table.size();
+  short_ = nchunks_ <= glx::kGradShortChunks && chunk <= glx::kGradShortBytes;
+  shortClip_ = short_ && nchunks_ <= kShortClipChunks;
+  streamed_ = std::max(0, nchunks_ - (int)(kCachedBytes / chunk));
   grid_ = (int)std::max<size_t>(1, std::min(table.size(), groups));
   if (nchunks_ > 0) {
     const size_t n = table.size() * sizeof(glx::GradChunk);
@@ -134,47 +147,56 @@ GradientList::~GradientList() {
   if (chunks_ != nullptr) (void)hipFree(chunks_);
 }
 
-void GradientList::powerSum(double p, void* sum, void* workspace, hipStream_t s) const {
-  const int kind = kindOf(p);
-  GLX_ENFORCE(sum != nullptr && workspace != nullptr, "gradients: null pointer");
-  checkOut(sum, GLX_FLOAT64);
+void GradientList::sum(int kind, bool root, int streamed, void* out, int outDtype,
+                       void* workspace, hipStream_t s) const {
+  GLX_ENFORCE(out != nullptr && (short_ || workspace != nullptr), "gradients: null pointer");
+  checkOut(out, outDtype);
   checkOut(workspace, GLX_FLOAT64);
   DeviceScope scope(device_);
+  if (short_) {
+    GLX_HIP_CHECK(
+        glx::launch_short(kind, chunks_, nchunks_, false, 0, root, out, outDtype, s));
+    return;
+  }
   double* part = (double*)workspace;
-  GLX_HIP_CHECK(glx::launch_power_partials(kind, chunks_, nchunks_, grid_, part, s));
-  GLX_HIP_CHECK(glx::launch_power_finish(kind, part, grid_, false, sum, GLX_FLOAT64, s));
+  GLX_HIP_CHECK(
+      glx::launch_power_partials(kind, chunks_, nchunks_, streamed, grid_, part, s));
+  GLX_HIP_CHECK(glx::launch_power_finish(kind, part, grid_, root, out, outDtype, s));
+}
+
+void GradientList::powerSum(double p, void* out, void* workspace, hipStream_t s) const {
+  sum(kindOf(p), false, streamed_, out, GLX_FLOAT64, workspace, s);  // a clip will follow
 }
 
 void GradientList::norm(double p, void* out, int outDtype, void* workspace,
                         hipStream_t s) const {
-  const int kind = kindOf(p);
-  GLX_ENFORCE(out != nullptr && workspace != nullptr, "gradients: null pointer");
-  checkOut(out, outDtype);
-  checkOut(workspace, GLX_FLOAT64);
-  DeviceScope scope(device_);
-  double* part = (double*)workspace;
-  GLX_HIP_CHECK(glx::launch_power_partials(kind, chunks_, nchunks_, grid_, part, s));
-  GLX_HIP_CHECK(glx::launch_power_finish(kind, part, grid_, true, out, outDtype, s));
+  sum(kindOf(p), true, nchunks_, out, outDtype, workspace, s);
 }
 
 void GradientList::clip(double maxNorm, double p, const void* powerSum, void* out, int outDtype,
                         void* workspace, hipStream_t s) const {
   const int kind = kindOf(p);
   GLX_ENFORCE(maxNorm >= 0, "gradients: max_norm is a number >= 0, not ", maxNorm);
-  GLX_ENFORCE(powerSum != nullptr || workspace != nullptr, "gradients: null workspace");
+  GLX_ENFORCE(powerSum != nullptr || shortClip_ || workspace != nullptr,
+              "gradients: null workspace");
   checkOut(out, outDtype);
   checkOut(powerSum != nullptr ? powerSum : workspace, GLX_FLOAT64);
   DeviceScope scope(device_);
   const double* part = (const double*)powerSum;
   int nparts = 1;
   if (part == nullptr) {
-    GLX_HIP_CHECK(glx::launch_power_partials(kind, chunks_, nchunks_, grid_, (double*)workspace,
-                                             s));
+    if (shortClip_) {
+      GLX_HIP_CHECK(
+          glx::launch_short(kind, chunks_, nchunks_, true, maxNorm, true, out, outDtype, s));
+      return;
+    }
+    GLX_HIP_CHECK(glx::launch_power_partials(kind, chunks_, nchunks_, streamed_, grid_,
+                                             (double*)workspace, s));
     part = (const double*)workspace;
     nparts = grid_;
   }
-  GLX_HIP_CHECK(glx::launch_clip(kind, chunks_, nchunks_, grid_, part, nparts, maxNorm, out,
-                                 outDtype, s));
+  GLX_HIP_CHECK(glx::launch_clip(kind, chunks_, nchunks_, part, nparts, maxNorm, out, outDtype,
+                                 s));
 }
 
 }  // namespace gloo

@@ -20,21 +20,30 @@ struct GradChunk {
   uint32_t dtype;
 };
 
+// The most chunks, of kGradShortBytes at most, that one workgroup does alone.
+constexpr int kGradShortChunks = 64;
+constexpr size_t kGradShortBytes = 4 << 10;
+
 constexpr int kGradNorm1 = 0, kGradNorm2 = 1, kGradNormInf = 2;
 
 // part[b] = sum of |x|^p (maximum for inf) over workgroup b's chunks, in
-// double.  grid workgroups; part has grid words.
-hipError_t launch_power_partials(int kind, const GradChunk* chunks, int nchunks, int grid,
-                                 double* part, hipStream_t s);
+// double.  grid workgroups; part has grid words.  The first `streamed` chunks are
+// read past the caches, the others to stay there for a clip.
+hipError_t launch_power_partials(int kind, const GradChunk* chunks, int nchunks, int streamed,
+                                 int grid, double* part, hipStream_t s);
 // The fold of nparts partials: the power sum itself (root = false, out double)
 // or the norm (root = true, out float or double by outDtype).
 hipError_t launch_power_finish(int kind, const double* part, int nparts, bool root, void* out,
                                int outDtype, hipStream_t s);
 // dst = x * min(1, maxNorm / (norm + 1e-6)) over all chunks, the norm folded
 // from the partials; the norm to `out` if not null.
-hipError_t launch_clip(int kind, const GradChunk* chunks, int nchunks, int grid,
-                       const double* part, int nparts, double maxNorm, void* out, int outDtype,
-                       hipStream_t s);
+hipError_t launch_clip(int kind, const GradChunk* chunks, int nchunks, const double* part,
+                       int nparts, double maxNorm, void* out, int outDtype, hipStream_t s);
+// Power sum or norm (root) to `out` if not null, and with `clip` the clipping
+// too (root is true then), in one launch of one workgroup.  At most
+// kGradShortChunks chunks of at most kGradShortBytes.
+hipError_t launch_short(int kind, const GradChunk* chunks, int nchunks, bool clip,
+                        double maxNorm, bool root, void* out, int outDtype, hipStream_t s);
 
 }  // namespace glx
 
@@ -67,16 +76,22 @@ class GradientList {
   GradientList& operator=(const GradientList&) = delete;
 
   int device() const { return device_; }
-  size_t workspaceBytes() const { return (size_t)grid_ * sizeof(double); }
+  size_t workspaceBytes() const { return shortClip_ ? 0 : (size_t)grid_ * sizeof(double); }
   void powerSum(double p, void* sum, void* workspace, hipStream_t s) const;
   void norm(double p, void* out, int outDtype, void* workspace, hipStream_t s) const;
   void clip(double maxNorm, double p, const void* powerSum, void* out, int outDtype,
             void* workspace, hipStream_t s) const;
 
  private:
+  void sum(int kind, bool root, int streamed, void* out, int outDtype, void* workspace,
+           hipStream_t s) const;
+
   int device_ = 0;
-  int grid_ = 1;
+  int grid_ = 1;            // workgroups of the sum, and partials
+  bool short_ = false;      // one workgroup sums it all
+  bool shortClip_ = false;  // and clips it
   int nchunks_ = 0;
+  int streamed_ = 0;        // chunks that a clip will not find in the cache anyway
   glx::GradChunk* chunks_ = nullptr;  // device memory
 };
 

@@ -7,10 +7,12 @@ data-parallel program does with the buffers its allreduce returns.
 import ctypes
 
 from . import _lib
-from .algorithms import FLOAT32, FLOAT64, _stream_ptr, torch_dtype_code
+from .algorithms import FLOAT32, FLOAT64, torch_dtype_code
 from .errors import check, check_handle
+from .streams import as_torch_stream, current_stream_ptr
 
 lib = _lib.lib
+torch = _lib.torch
 
 
 def _dense(t):
@@ -43,7 +45,6 @@ class Gradients:
     holding it, runs."""
 
     def __init__(self, grads, outs=None):
-        import torch
         grads = list(grads)
         outs = None if outs is None else list(outs)
         if outs is not None and len(outs) != len(grads):
@@ -90,53 +91,54 @@ class Gradients:
             raise ValueError("%s: one %s on %s" % (what, dtype, self.device))
         return t.data_ptr()
 
-    def _call(self, fn, dtype, out, stream, args):
-        """fn(handle, *args(out pointer, workspace pointer), stream)."""
-        import torch
+    def _begin(self, dtype, out):
+        """(handle, result tensor, workspace, its pointer or None, stream) of
+        one call on the current stream, which what is allocated here belongs to."""
         if self._h is None:
             raise ValueError("Gradients: closed")
-        if stream is None:
-            stream = torch.cuda.current_stream(self.device)
-        elif stream != torch.cuda.current_stream(self.device):
-            # what is allocated here belongs to the stream that uses it
-            own = torch.cuda.ExternalStream(stream, self.device) if isinstance(stream, int) \
-                else stream
-            with torch.cuda.stream(own):
-                return self._call(fn, dtype, out, None, args)
         if out is None:
             out = torch.empty((), dtype=dtype, device=self.device)
         else:
             self._scalar(out, dtype, "out")
-        ws = torch.empty(self._ws, dtype=torch.float64, device=self.device)
-        check(fn(self._h, *args(out.data_ptr(), ws.data_ptr()), _stream_ptr(stream)),
-              "Gradients")
-        return out
+        ws = torch.empty(self._ws, dtype=torch.float64, device=self.device) if self._ws else None
+        return (self._h, out, ws, None if ws is None else ws.data_ptr(),
+                current_stream_ptr(self.device))
 
     def power_sum(self, p=2.0, out=None, stream=None):
         """The sum of |x|^p over all gradients (the maximum of |x| for
         p = inf; p is 1, 2 or inf), accumulated in and returned as float64.
         Ranks holding shards allreduce it (SUM; MAX for inf) and give it to
         clip_norm."""
-        import torch
-        return self._call(lib.glx_gradients_power_sum, torch.float64, out, stream,
-                          lambda o, ws: (float(p), o, ws))
+        if stream is not None:
+            with torch.cuda.stream(as_torch_stream(stream, self.device)):
+                return self.power_sum(p, out)
+        h, out, ws, wp, s = self._begin(torch.float64, out)
+        check(lib.glx_gradients_power_sum(h, p, out.data_ptr(), wp, s), "Gradients")
+        return out
 
     def norm(self, p=2.0, out=None, stream=None):
         """The p-norm of all gradients together: float32, or float64 if one
         of them is."""
-        return self._call(lib.glx_gradients_norm, self.dtype, out, stream,
-                          lambda o, ws: (float(p), o, self._code, ws))
+        if stream is not None:
+            with torch.cuda.stream(as_torch_stream(stream, self.device)):
+                return self.norm(p, out)
+        h, out, ws, wp, s = self._begin(self.dtype, out)
+        check(lib.glx_gradients_norm(h, p, out.data_ptr(), self._code, wp, s), "Gradients")
+        return out
 
     def clip_norm(self, max_norm, p=2.0, power_sum=None, out=None, stream=None):
         """Scale every gradient by min(1, max_norm / (norm + 1e-6)), in place
         or into outs, and return the norm (as norm() does): the list's own,
         or that of power_sum (a float64 on the device).  A NaN norm makes
         every gradient NaN, an infinite one 0 (NaN where it was infinite)."""
-        import torch
+        if stream is not None:
+            with torch.cuda.stream(as_torch_stream(stream, self.device)):
+                return self.clip_norm(max_norm, p, power_sum, out)
         total = None if power_sum is None else self._scalar(power_sum, torch.float64, "power_sum")
-        return self._call(lib.glx_gradients_clip, self.dtype, out, stream,
-                          lambda o, ws: (float(max_norm), float(p), total, o,
-                                         self._code, ws))
+        h, out, ws, wp, s = self._begin(self.dtype, out)
+        check(lib.glx_gradients_clip(h, max_norm, p, total, out.data_ptr(), self._code, wp, s),
+              "Gradients")
+        return out
 
     def close(self):
         """Free the handle (its work, and graphs holding it, must be done)."""

@@ -20,51 +20,55 @@ read nor written.
 import ctypes
 
 from . import _lib
-from .algorithms import _stream_ptr, torch_dtype_code
+from .algorithms import BFLOAT16, FLOAT16, FLOAT32
 from .errors import check
+from .streams import as_torch_stream, current_stream_ptr
 
 lib = _lib.lib
+torch = _lib.torch
+_CODES = {} if torch is None else {
+    torch.float32: FLOAT32, torch.float16: FLOAT16, torch.bfloat16: BFLOAT16}
 
 
 def payload_bytes(n):
-    """Bytes of the payload of n elements."""
+    """Bytes of the payload of n elements (glx_mx_payload_bytes)."""
     if not 0 <= n <= 1 << 60:
         raise ValueError("payload_bytes: %d elements" % n)
-    return int(lib.glx_mx_payload_bytes(n))
+    return ((n + 31) // 32 * 17 + 15) // 16 * 16
 
 
-def _check(t, what, device, dtype=None):
+def _check(t, what, device=None):
     if not t.is_cuda or (device is not None and t.device != device):
         raise ValueError("mx: %s is on %s" % (what, t.device))
     if not t.is_contiguous():
         raise ValueError("mx: %s is not contiguous" % what)
-    if dtype is not None and t.dtype != dtype:
-        raise TypeError("mx: %s is %s, not %s" % (what, t.dtype, dtype))
 
 
-def _check_payload(t, n, what, device):
-    import torch
-    _check(t, what, device, torch.uint8)
-    if t.numel() < payload_bytes(n):
-        raise ValueError("mx: %s has %d bytes, %d elements need %d"
-                         % (what, t.numel(), n, payload_bytes(n)))
+def _code(t, what):
+    code = _CODES.get(t.dtype)
+    if code is None:
+        raise TypeError("mx: %s is %s, not float32, float16 or bfloat16" % (what, t.dtype))
+    return code
 
 
-def _stream(stream, device):
-    if stream is None:
-        import torch
-        stream = torch.cuda.current_stream(device)
-    return _stream_ptr(stream)
+def _payload_ptr(t, need, device, what="payload"):
+    _check(t, what, device)
+    if t.dtype != torch.uint8:
+        raise TypeError("mx: %s is %s, not uint8" % (what, t.dtype))
+    if t.numel() < need:
+        raise ValueError("mx: %s has %d bytes of the %d needed" % (what, t.numel(), need))
+    return t.data_ptr()
 
 
-def _new_payload(n, device, stream):
-    import torch
-    if stream is None:
-        return torch.empty(payload_bytes(n), dtype=torch.uint8, device=device)
-    if isinstance(stream, int):
-        stream = torch.cuda.ExternalStream(stream, device)
-    with torch.cuda.stream(stream):  # the memory belongs to the stream that uses it
-        return torch.empty(payload_bytes(n), dtype=torch.uint8, device=device)
+def _residual_ptr(t, n, device, what):
+    if t is None:
+        return None
+    _check(t, what, device)
+    if t.dtype != torch.float32:
+        raise TypeError("mx: %s is %s, not float32" % (what, t.dtype))
+    if t.numel() != n:
+        raise ValueError("mx: %s has %d elements, x %d" % (what, t.numel(), n))
+    return t.data_ptr()
 
 
 def quantize(x, payload=None, residual=None, residual_out=None, stream=None):
@@ -72,55 +76,55 @@ def quantize(x, payload=None, residual=None, residual_out=None, stream=None):
     (float32, as many elements) of x + residual.  residual_out receives what
     the payload leaves out, to be added to the next message; it may be
     `residual` itself.  Returns the payload (allocated unless given)."""
-    import torch
-    _check(x, "x", None)
-    n = x.numel()
-    for t, what in ((residual, "residual"), (residual_out, "residual_out")):
-        if t is not None:
-            _check(t, what, x.device, torch.float32)
-            if t.numel() != n:
-                raise ValueError("mx: %s has %d elements, x %d" % (what, t.numel(), n))
-    code = torch_dtype_code(x)
+    if stream is not None:
+        with torch.cuda.stream(as_torch_stream(stream, x.device)):
+            return quantize(x, payload, residual, residual_out)
+    _check(x, "x")
+    code, n, device = _code(x, "x"), x.numel(), x.device
+    need = payload_bytes(n)
     if payload is None:
-        payload = _new_payload(n, x.device, stream)
-    _check_payload(payload, n, "payload", x.device)
-    check(lib.glx_mx_quantize(code, payload.data_ptr(), x.data_ptr(),
-                              None if residual is None else residual.data_ptr(),
-                              None if residual_out is None else residual_out.data_ptr(),
-                              n, _stream(stream, x.device)), "mx.quantize")
+        payload = torch.empty(need, dtype=torch.uint8, device=device)
+    check(lib.glx_mx_quantize(code, _payload_ptr(payload, need, device), x.data_ptr(),
+                              _residual_ptr(residual, n, device, "residual"),
+                              _residual_ptr(residual_out, n, device, "residual_out"),
+                              n, current_stream_ptr(device)), "mx.quantize")
     return payload
 
 
-def _sources(payloads, n, device):
-    payloads = list(payloads)
-    for j, t in enumerate(payloads):
-        _check_payload(t, n, "payload %d" % j, device)
-    return (ctypes.c_void_p * len(payloads))(*[t.data_ptr() for t in payloads]), len(payloads)
+def _sources(payloads, need, device):
+    ptrs = [_payload_ptr(t, need, device, "payload %d" % j) for j, t in enumerate(payloads)]
+    return (ctypes.c_void_p * len(ptrs))(*ptrs), len(ptrs)
 
 
 def reduce_n(dst, payloads, scale=1.0, stream=None):
     """dst = scale * the left fold of 1..16 payloads of dst.numel() elements,
     in float32, rounded once to dst's type (float32, float16, bfloat16)."""
-    _check(dst, "dst", None)
-    arr, k = _sources(payloads, dst.numel(), dst.device)
-    check(lib.glx_mx_reduce_n(torch_dtype_code(dst), dst.data_ptr(), arr, k, dst.numel(),
-                              float(scale), _stream(stream, dst.device)), "mx.reduce_n")
+    if stream is not None:
+        with torch.cuda.stream(as_torch_stream(stream, dst.device)):
+            return reduce_n(dst, payloads, scale)
+    _check(dst, "dst")
+    code, n, device = _code(dst, "dst"), dst.numel(), dst.device
+    arr, k = _sources(payloads, payload_bytes(n), device)
+    check(lib.glx_mx_reduce_n(code, dst.data_ptr(), arr, k, n, scale,
+                              current_stream_ptr(device)), "mx.reduce_n")
     return dst
 
 
 def dequantize(dst, payload, stream=None):
     """dst = the values of a payload of dst.numel() elements."""
-    return reduce_n(dst, [payload], stream=stream)
+    return reduce_n(dst, (payload,), 1.0, stream)
 
 
 def requantize_n(payload, payloads, n, scale=1.0, stream=None):
     """payload = the payload of scale * the left fold of 1..16 payloads of n
     elements (in float32): one hop of a compressed exchange.  payload may be
     one of the sources."""
-    if payload is None:
-        raise ValueError("mx: requantize_n needs a payload to write")
-    _check_payload(payload, n, "payload", None)
-    arr, k = _sources(payloads, n, payload.device)
-    check(lib.glx_mx_requantize_n(payload.data_ptr(), arr, k, int(n), float(scale),
-                                  _stream(stream, payload.device)), "mx.requantize_n")
+    if stream is not None:
+        with torch.cuda.stream(as_torch_stream(stream, payload.device)):
+            return requantize_n(payload, payloads, n, scale)
+    need, device = payload_bytes(n), payload.device
+    out = _payload_ptr(payload, need, device)
+    arr, k = _sources(payloads, need, device)
+    check(lib.glx_mx_requantize_n(out, arr, k, n, scale, current_stream_ptr(device)),
+          "mx.requantize_n")
     return payload

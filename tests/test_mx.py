@@ -118,7 +118,7 @@ def dev(a):
 
 @pytest.mark.parametrize("n", [0, 1, 31, 32, 33, 255, 256, 257, 512, 4099, (1 << 33) + 1])
 def test_payload_bytes(n):
-    assert mx.payload_bytes(n) == mx_bytes(n)
+    assert mx.payload_bytes(n) == mx_bytes(n) == _lib.lib.glx_mx_payload_bytes(n)
 
 
 def test_payload_bytes_refuses():
@@ -340,7 +340,7 @@ def test_quantize_refuses():
         mx.quantize(x, p, residual=x.half())
     with pytest.raises(ValueError, match="elements"):
         mx.quantize(x, p, residual=x[:63])
-    with pytest.raises(gloo_amd.EnforceNotMet):
+    with pytest.raises(TypeError, match="float64"):
         mx.quantize(x.double(), p)
     with pytest.raises(gloo_amd.EnforceNotMet, match="16-byte"):
         mx.quantize(x, torch.zeros(64, dtype=torch.uint8, device="cuda")[8:56])
@@ -456,10 +456,10 @@ def test_fold_refuses():
         mx.reduce_n(x, [x.view(torch.uint8)[:48]])
     with pytest.raises(gloo_amd.EnforceNotMet, match="finite"):
         mx.reduce_n(x, [p], scale=float("nan"))
-    with pytest.raises(gloo_amd.EnforceNotMet):
+    with pytest.raises(TypeError, match="float64"):
         mx.reduce_n(x.double(), [p])
-    with pytest.raises(ValueError):
-        mx.requantize_n(None, [p], 64)
+    with pytest.raises(ValueError, match="bytes"):
+        mx.requantize_n(p, [p], 128)
 
 
 # ---- streams, graphs, length -------------------------------------------------
