@@ -34,21 +34,12 @@ int kindOf(double p) {
   return glx::kGradNormInf;
 }
 
-void checkOut(const void* out, int dtype) {
-  GLX_ENFORCE(dtype == GLX_FLOAT32 || dtype == GLX_FLOAT64,
-              "gradients: the norm is written as float32 or float64");
-  GLX_ENFORCE((uintptr_t)out % (dtype == GLX_FLOAT32 ? 4 : 8) == 0,
-              "gradients: misaligned scalar");
-}
+bool aligned(const void* p, int dtype) { return (uintptr_t)p % elementSize(dtype) == 0; }
 
-struct Span {
-  uintptr_t at, end;
-  size_t tensor;
-  bool out;
-};
+using Span = GradientList::Span;
 
 // Every byte is written by at most one tensor, and none that another reads.
-void checkOverlap(std::vector<Span> spans) {
+void checkOverlap(std::vector<Span>& spans) {
   std::sort(spans.begin(), spans.end(),
             [](const Span& a, const Span& b) { return a.at < b.at; });
   for (size_t i = 1; i < spans.size(); i++) {
@@ -80,7 +71,7 @@ DeviceScope::~DeviceScope() {
 
 GradientList::GradientList(const std::vector<void*>& grads, const std::vector<void*>& outs,
                            const std::vector<size_t>& counts, const std::vector<int>& dtypes) {
-  std::vector<Span> spans;
+  std::vector<Span>& spans = spans_;
   size_t bytes = 0;
   for (size_t i = 0; i < grads.size(); i++) {
     const size_t es = elementSize(dtypes[i]);
@@ -147,11 +138,34 @@ GradientList::~GradientList() {
   if (chunks_ != nullptr) (void)hipFree(chunks_);
 }
 
+// A scalar in device memory, outside the tensors.
+void GradientList::checkScalar(const void* p, int dtype, const char* what) const {
+  GLX_ENFORCE(dtype == GLX_FLOAT32 || dtype == GLX_FLOAT64, "gradients: ", what,
+              " is a float32 or float64");
+  GLX_ENFORCE(p != nullptr && aligned(p, dtype), "gradients: ", what, " is null or misaligned");
+  const uintptr_t at = (uintptr_t)p, end = at + elementSize(dtype);
+  // spans_ is sorted and without overlap: only the last one that begins before
+  // the scalar's end can reach it
+  auto i = std::lower_bound(spans_.begin(), spans_.end(), end,
+                            [](const Span& s, uintptr_t e) { return s.at < e; });
+  GLX_ENFORCE(i == spans_.begin() || (i - 1)->end <= at, "gradients: ", what,
+              " lies in a tensor's memory");
+}
+
+// The partials' memory, apart from the result.
+void GradientList::checkWorkspace(const void* p, const void* scalar) const {
+  GLX_ENFORCE(p != nullptr && aligned(p, GLX_FLOAT64),
+              "gradients: workspace is null or misaligned");
+  const uintptr_t w = (uintptr_t)p, end = w + (size_t)grid_ * sizeof(double);
+  const uintptr_t q = (uintptr_t)scalar;
+  GLX_ENFORCE(scalar == nullptr || q < w || q >= end,
+              "gradients: a scalar lies in the workspace");
+}
+
 void GradientList::sum(int kind, bool root, int streamed, void* out, int outDtype,
                        void* workspace, hipStream_t s) const {
-  GLX_ENFORCE(out != nullptr && (short_ || workspace != nullptr), "gradients: null pointer");
-  checkOut(out, outDtype);
-  checkOut(workspace, GLX_FLOAT64);
+  checkScalar(out, outDtype, "out");
+  if (!short_) checkWorkspace(workspace, out);
   DeviceScope scope(device_);
   if (short_) {
     GLX_HIP_CHECK(
@@ -177,10 +191,15 @@ void GradientList::clip(double maxNorm, double p, const void* powerSum, void* ou
                         void* workspace, hipStream_t s) const {
   const int kind = kindOf(p);
   GLX_ENFORCE(maxNorm >= 0, "gradients: max_norm is a number >= 0, not ", maxNorm);
-  GLX_ENFORCE(powerSum != nullptr || shortClip_ || workspace != nullptr,
-              "gradients: null workspace");
-  checkOut(out, outDtype);
-  checkOut(powerSum != nullptr ? powerSum : workspace, GLX_FLOAT64);
+  if (out != nullptr) checkScalar(out, outDtype, "norm");
+  if (powerSum != nullptr) {
+    checkScalar(powerSum, GLX_FLOAT64, "power_sum");
+    const uintptr_t q = (uintptr_t)powerSum, o = (uintptr_t)out;
+    GLX_ENFORCE(out == nullptr || o + elementSize(outDtype) <= q || o >= q + sizeof(double),
+                "gradients: norm and power_sum share memory");
+  } else if (!shortClip_) {
+    checkWorkspace(workspace, out);
+  }
   DeviceScope scope(device_);
   const double* part = (const double*)powerSum;
   int nparts = 1;

@@ -69,6 +69,12 @@ int deviceOf(const void* p);
 // at once, each with a workspace of its own.
 class GradientList {
  public:
+  struct Span {  // memory of a tensor
+    uintptr_t at, end;
+    size_t tensor;
+    bool out;
+  };
+
   GradientList(const std::vector<void*>& grads, const std::vector<void*>& outs,
                const std::vector<size_t>& counts, const std::vector<int>& dtypes);
   ~GradientList();
@@ -86,6 +92,10 @@ class GradientList {
   void sum(int kind, bool root, int streamed, void* out, int outDtype, void* workspace,
            hipStream_t s) const;
 
+  void checkScalar(const void* p, int dtype, const char* what) const;
+  void checkWorkspace(const void* p, const void* scalar) const;
+
+  std::vector<Span> spans_;  // sorted
   int device_ = 0;
   int grid_ = 1;            // workgroups of the sum, and partials
   bool short_ = false;      // one workgroup sums it all

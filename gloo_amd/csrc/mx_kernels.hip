@@ -85,9 +85,14 @@ __device__ __forceinline__ uint32_t max_with(uint32_t v) {
   return v > o ? v : o;
 }
 
+// The conversions take the scale as a float of which they use the exponent
+// field, with E8M0's meaning throughout: 0 is 2^-127, 255 makes every value NaN
+// (all 256 bytes checked, with halfway points and their neighbours).
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+
 template <int SEL>
-__device__ __forceinline__ uint32_t two_codes(uint32_t c, float a, float b) {
-  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, a, b, 1.f, SEL);
+__device__ __forceinline__ uint32_t two_codes(uint32_t c, float a, float b, float scale) {
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, a, b, scale, SEL);
 }
 
 // A block of which this lane holds E values: its scale byte, and the lane's
@@ -110,38 +115,33 @@ __device__ __forceinline__ Block encode(const float (&y)[E]) {
   const uint32_t e = top >> 23;
   if (e == 255) return {0, 255};
   const uint32_t s = e > 2 ? e - 2 : 0;
-  const float inv = __uint_as_float((254 - s) << 23);  // 2^(127 - s): s <= 252
+  const float sc = scale_of(s);
   uint32_t c = 0;
-  c = two_codes<0>(c, y[0] * inv, y[1] * inv);
-  c = two_codes<1>(c, y[2] * inv, y[3] * inv);
+  c = two_codes<0>(c, y[0], y[1], sc);
+  c = two_codes<1>(c, y[2], y[3], sc);
   if constexpr (E == 8) {
-    c = two_codes<2>(c, y[4] * inv, y[5] * inv);
-    c = two_codes<3>(c, y[6] * inv, y[7] * inv);
+    c = two_codes<2>(c, y[4], y[5], sc);
+    c = two_codes<3>(c, y[6], y[7], sc);
   }
   return {c, s};
 }
 
 template <int SEL>
-__device__ __forceinline__ void two_values(uint32_t c, float* v) {
-  const v2f p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, SEL);
+__device__ __forceinline__ void two_values(uint32_t c, float scale, float* v) {
+  const v2f p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, SEL);
   v[0] = p[0];
   v[1] = p[1];
 }
 
-// The unscaled values of E codes.
+// The values of E codes.
 template <int E>
-__device__ __forceinline__ void decode(uint32_t c, float (&v)[E]) {
-  two_values<0>(c, v);
-  two_values<1>(c, v + 2);
+__device__ __forceinline__ void decode(uint32_t c, float scale, float (&v)[E]) {
+  two_values<0>(c, scale, v);
+  two_values<1>(c, scale, v + 2);
   if constexpr (E == 8) {
-    two_values<2>(c, v + 4);
-    two_values<3>(c, v + 6);
+    two_values<2>(c, scale, v + 4);
+    two_values<3>(c, scale, v + 6);
   }
-}
-
-// 2^(s - 127), subnormal for s = 0, NaN for s = 255.
-__device__ __forceinline__ float scale_of(uint32_t s) {
-  return __uint_as_float((s << 23) | (s == 0 || s == 255 ? 0x00400000u : 0u));
 }
 
 // E codes of a lane, as they lie in a payload.
@@ -235,12 +235,9 @@ __device__ __forceinline__ void quantize_tile(char* payload, const typename T::S
     put_block(payload, nb, tile, t, b);
     if constexpr (RES_OUT) {
       float v[E];
-      decode<E>(b.code, v);
-      const float sc = scale_of(b.scale);
+      decode<E>(b.code, scale_of(b.scale), v);
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        v[e] = b.scale == 255 ? 0.f : __builtin_fmaf(-v[e], sc, y[u][e]);  // exact
-      }
+      for (int e = 0; e < E; e++) v[e] = b.scale == 255 ? 0.f : y[u][e] - v[e];  // exact
       store<F32, E, FULL>(residualOut, t * E, tile.left, v);
     }
   }
@@ -286,18 +283,15 @@ struct Part {
       scale[j] = s[t / kLanes];
     }
   }
-  // the left fold, times scale
+  // the left fold, times `by`
   __device__ __forceinline__ void fold(float by, float (&acc)[E]) const {
+    decode<E>(code[0], scale_of(scale[0]), acc);
 #pragma unroll
-    for (int j = 0; j < K; j++) {
+    for (int j = 1; j < K; j++) {
       float v[E];
-      decode<E>(code[j], v);
-      const float sc = scale_of(scale[j]);
+      decode<E>(code[j], scale_of(scale[j]), v);
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        // v * sc is exact: the fma rounds only the sum
-        acc[e] = j == 0 ? v[e] * sc : __builtin_fmaf(v[e], sc, acc[e]);
-      }
+      for (int e = 0; e < E; e++) acc[e] = __fadd_rn(acc[e], v[e]);
     }
 #pragma unroll
     for (int e = 0; e < E; e++) acc[e] = __fmul_rn(acc[e], by);

@@ -58,12 +58,16 @@ class Gradients:
             codes.append(code)
             if not t.is_cuda or t.device != grads[0].device:
                 raise ValueError("gradient %d is on %s" % (i, t.device))
+            if t.is_neg():
+                raise ValueError("gradient %d is a negated view" % i)
             if t.numel() and not _dense(t):
                 raise ValueError("gradient %d has gaps or overlaps in its memory (strides %s)"
                                  % (i, tuple(t.stride())))
             if outs is None:
                 continue
             o = outs[i]
+            if o.is_neg():
+                raise ValueError("out %d is a negated view" % i)
             if o.dtype != t.dtype:
                 raise TypeError("out %d is %s, its gradient %s" % (i, o.dtype, t.dtype))
             if o.device != t.device or o.shape != t.shape or (

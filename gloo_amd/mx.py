@@ -40,8 +40,8 @@ def payload_bytes(n):
 def _check(t, what, device=None):
     if not t.is_cuda or (device is not None and t.device != device):
         raise ValueError("mx: %s is on %s" % (what, t.device))
-    if not t.is_contiguous():
-        raise ValueError("mx: %s is not contiguous" % what)
+    if not t.is_contiguous() or t.is_neg():
+        raise ValueError("mx: %s is not contiguous, or a negated view" % what)
 
 
 def _code(t, what):

@@ -388,6 +388,64 @@ def test_out_arguments():
 
 
 @gpu
+@pytest.mark.parametrize("n", [10, 1 << 20])  # one workgroup, and many
+def test_scalars_apart_from_the_tensors(n):
+    """What a call writes beside the tensors lies outside what it reads."""
+    x = torch.ones(n, device="cuda", dtype=torch.float64)
+    g = Gradients([x[1:-1]])
+    s = g.power_sum()
+    for out in (x[1], x[n // 2], x[n - 2]):
+        with pytest.raises(gloo_amd.EnforceNotMet, match="lies in a tensor"):
+            g.norm(out=out)
+        with pytest.raises(gloo_amd.EnforceNotMet, match="lies in a tensor"):
+            g.clip_norm(1.0, power_sum=out)
+    with pytest.raises(gloo_amd.EnforceNotMet, match="share memory"):
+        g.clip_norm(1.0, power_sum=s, out=s)
+    assert float(g.norm(out=x[0])) == float(g.norm(out=x[n - 1])) == float(np.sqrt(n - 2.0))
+    ws = torch.zeros(1 << 14, device="cuda", dtype=torch.float64)
+    if _lib.lib.glx_gradients_workspace_bytes(g._h):
+        for at in (None, ws.data_ptr() + 4):
+            assert _lib.lib.glx_gradients_norm(g._h, 2.0, s.data_ptr(), 6, at, None) == \
+                _lib.ERR_ENFORCE
+        assert _lib.lib.glx_gradients_norm(g._h, 2.0, ws.data_ptr() + 8, 6, ws.data_ptr(),
+                                           None) == _lib.ERR_ENFORCE
+    assert _lib.lib.glx_gradients_norm(g._h, 2.0, s.data_ptr(), 5 + 2, ws.data_ptr(), None) == \
+        _lib.ERR_ENFORCE
+    assert bool((x[1:-1] == 1).all())
+    # no norm wanted: the clip alone
+    assert _lib.lib.glx_gradients_clip(g._h, 0.5, float("inf"), None, None, 0, ws.data_ptr(),
+                                       None) == 0
+    torch.cuda.synchronize()
+    assert bool(((x[1:-1] - 0.5).abs() <= 1e-6).all()) and float(x[0]) != 0.5
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+def test_clip_of_subnormal_values(dtype):
+    """Values down to the type's smallest, clipped by a norm that one large value
+    makes: rounded to the subnormal grid, not flushed."""
+    t = DTYPES[dtype]
+    f = torch.finfo(t)
+    tiny = f.smallest_normal * f.eps
+    v = torch.arange(1, 3000, dtype=torch.float64) * tiny
+    x = torch.cat([v, -v, torch.tensor([4.0], dtype=torch.float64)]).to(t).cuda()
+    was = x.clone()
+    total = exact_norm([was], 2)
+    out = torch.empty_like(x)
+    Gradients([x], outs=[out]).clip_norm(total / 3)
+    check_clipped(out, was, total, total / 3)
+    assert int(out.count_nonzero()) > 5000 - 4
+
+
+@gpu
+def test_negated_views_are_refused():
+    x = torch._neg_view(torch.ones(8, device="cuda"))
+    for call in (lambda: Gradients([x]), lambda: gloo_amd.mx.quantize(x)):
+        with pytest.raises(ValueError, match="negated"):
+            call()
+
+
+@gpu
 def test_keeps_the_memory_it_was_given():
     """A parameter whose gradient is replaced: the handle still has the old one."""
     w = torch.nn.Parameter(torch.zeros(1000, device="cuda"))
@@ -407,10 +465,14 @@ def test_streams():
     g = Gradients(views)
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
-    for stream in (s, s.cuda_stream):
+    for stream in (s, s.cuda_stream, torch.cuda.default_stream()):
         n = g.norm(stream=stream)
-        s.synchronize()
+        torch.cuda.synchronize()
         check_norm(n, views, 2)
+    with torch.cuda.stream(s):  # the default stream by its handle, from another current one
+        n = g.norm(stream=0)
+    torch.cuda.synchronize()
+    check_norm(n, views, 2)
 
 
 @gpu
