@@ -14,7 +14,7 @@
 // The lanes of a block (8 or 4) find its maximum in two or three DPP exchanges,
 // without shared memory.  One pass per lane, no loop over a capped grid: the
 // loop cost 10 to 20 % everywhere (256 MiB of bf16 quantised: 65 us with 4
-// workgroups a CU, 57 us with one pass).  Loads and stores are nontemporal.
+// workgroups a CU, 57 us with one pass).  Float loads and stores are nontemporal.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -169,7 +169,10 @@ struct Tile {
         left((uint32_t)(n - first * E)) {}
 };
 
-// Codes and scale of lane t of the tile.
+// Codes and scale of lane t of the tile.  Plain stores, unlike those of floats:
+// what sends or opens the payload next finds it in the Infinity Cache (256 MiB
+// of bf16 quantised and opened 102 instead of 109 us, four payloads folded into
+// one and opened 144 instead of 151; the quantisation by itself is 2 % slower).
 template <int E, int U>
 __device__ __forceinline__ void put_block(char* payload, size_t nb, const Tile<E, U>& tile,
                                           uint32_t t, Block b) {
@@ -177,7 +180,7 @@ __device__ __forceinline__ void put_block(char* payload, size_t nb, const Tile<E
   constexpr uint32_t kLanes = Tile<E, U>::kLanes;
   GLX_GLOBAL C* code = (GLX_GLOBAL C*)payload + tile.first;
   GLX_GLOBAL char* scale = (GLX_GLOBAL char*)payload + nb * 16 + tile.first / kLanes;
-  __builtin_nontemporal_store((C)b.code, code + t);
+  code[t] = (C)b.code;
   if (t % kLanes == 0) scale[t / kLanes] = (char)b.scale;
 }
 
@@ -198,12 +201,13 @@ struct QuantizeShape {
   static constexpr int U = FEEDBACK ? 1 : 2;
 };
 
-// Folds into floats: one payload into 1 GiB of f32 238, 196, 217 us with U = 1,
-// 2, 4; four 283, 267, 276; eight 370, 382, 378.
-constexpr int kReduceParts = 2;
+// Folds into floats, 1 GiB of f32: one payload 227, 192, 216 us with U = 1, 2,
+// 4; four 285, 266, 276; eight 370, 387, 372 (into 256 MiB of bf16 128, 137, 132).
+template <int K>
+constexpr int kReduceParts = K <= 4 ? 2 : 1;
 
 // Folds into a payload, whose lanes do little but load: 128 Mi elements of one
-// payload 35, 32, 27 us with U = 1, 2, 4; four 66, 62, 59; eight 115, 117, 112.
+// payload 29, 25, 23 us with U = 2, 4, 8; four 59, 57, 58; eight 110, 101, 107.
 // From nine sources on four parts would not fit the registers.
 template <int K>
 constexpr int kRequantizeParts = K <= 8 ? 4 : 2;
@@ -321,7 +325,7 @@ template <typename T, int K, bool NT>
 __global__ __launch_bounds__(kBlock) void mx_reduce_n_kernel(typename T::S* dst, MxSources src,
                                                              size_t n, size_t nb, float scale,
                                                              size_t tile0) {
-  constexpr int E = 16 / sizeof(typename T::S), U = kReduceParts;
+  constexpr int E = 16 / sizeof(typename T::S), U = kReduceParts<K>;
   const Tile<E, U> tile(tile0 + blockIdx.x, n, nb);
   if (tile.full) {
     reduce_tile<T, K, NT, true>(dst, src, nb, scale, tile);
@@ -423,7 +427,7 @@ hipError_t reduce_k(void* dst, const MxSources& src, size_t n, float scale, hipS
   constexpr int E = 16 / sizeof(typename T::S);
   const size_t nb = mxBlocks(n);
   const bool nt = streaming(src, K);
-  return over_tiles(nb, E, kReduceParts, [&](dim3 grid, size_t tile0) {
+  return over_tiles(nb, E, kReduceParts<K>, [&](dim3 grid, size_t tile0) {
     if (K > 1 && nt) {
       hipLaunchKernelGGL((mx_reduce_n_kernel<T, K, (K > 1)>), grid, dim3(kBlock), 0, s,
                          (typename T::S*)dst, src, n, nb, scale, tile0);
