@@ -149,16 +149,16 @@ template <int E> struct Codes;
 template <> struct Codes<4> { using type = uint16_t; };
 template <> struct Codes<8> { using type = uint32_t; };
 
-// What a workgroup takes: kBlock * U lanes' parts from lane `first` (E elements
-// each) on.  Everything is addressed from there with 32 bits, from pointers
+// What a workgroup of N threads takes: N * U lanes' parts from lane `first` (E
+// elements each) on.  Everything is addressed from there with 32 bits, from pointers
 // that are the same for the whole wave.  Only the last tile is not full.  (No
 // 64-bit minimum of what is left and the tile's size: beside the comparison with
 // the size the compiler made of it a select on a stale condition bit, seen in
 // the assembly, and the tile counted as full.)
-template <int E, int U>
+template <int E, int U, int N>
 struct Tile {
   static constexpr uint32_t kLanes = 32 / E;  // of a block
-  static constexpr size_t kParts = (size_t)kBlock * U;
+  static constexpr size_t kParts = (size_t)N * U;
   size_t first;
   bool full;
   uint32_t lanes, left;  // lanes and elements there are, of a tile that is not full
@@ -173,11 +173,11 @@ struct Tile {
 // what sends or opens the payload next finds it in the Infinity Cache (256 MiB
 // of bf16 quantised and opened 102 instead of 109 us, four payloads folded into
 // one and opened 144 instead of 151; the quantisation by itself is 2 % slower).
-template <int E, int U>
-__device__ __forceinline__ void put_block(char* payload, size_t nb, const Tile<E, U>& tile,
+template <int E, int U, int N>
+__device__ __forceinline__ void put_block(char* payload, size_t nb, const Tile<E, U, N>& tile,
                                           uint32_t t, Block b) {
   using C = typename Codes<E>::type;
-  constexpr uint32_t kLanes = Tile<E, U>::kLanes;
+  constexpr uint32_t kLanes = Tile<E, U, N>::kLanes;
   GLX_GLOBAL C* code = (GLX_GLOBAL C*)payload + tile.first;
   GLX_GLOBAL char* scale = (GLX_GLOBAL char*)payload + nb * 16 + tile.first / kLanes;
   code[t] = (C)b.code;
@@ -205,6 +205,10 @@ struct QuantizeShape {
 // 4; four 285, 266, 276; eight 370, 387, 372 (into 256 MiB of bf16 128, 137, 132).
 template <int K>
 constexpr int kReduceParts = K <= 4 ? 2 : 1;
+// ... by 512 threads: with 256 the scale bytes of a 128-byte line belong to four
+// workgroups, and as many XCDs fetch it (1342 MB read for 1141 MB of eight
+// payloads): 370 us; 512 threads 354, 1024 382.  One payload 190, 180, 216.
+constexpr int kReduceThreads = 512;
 
 // Folds into a payload, whose lanes do little but load: 128 Mi elements of one
 // payload 29, 25, 23 us with U = 2, 4, 8; four 59, 57, 58; eight 110, 101, 107.
@@ -212,24 +216,24 @@ constexpr int kReduceParts = K <= 4 ? 2 : 1;
 template <int K>
 constexpr int kRequantizeParts = K <= 8 ? 4 : 2;
 
-template <typename T, bool RES_IN, bool RES_OUT, bool FULL, int E, int U>
+template <typename T, bool RES_IN, bool RES_OUT, bool FULL, int E, int U, int N>
 __device__ __forceinline__ void quantize_tile(char* payload, const typename T::S* x_,
                                               const float* residual_, float* residualOut_,
-                                              size_t nb, const Tile<E, U>& tile) {
+                                              size_t nb, const Tile<E, U, N>& tile) {
   const GLX_GLOBAL typename T::S* x = (const GLX_GLOBAL typename T::S*)x_ + tile.first * E;
   const GLX_GLOBAL float* residual = (const GLX_GLOBAL float*)residual_ + tile.first * E;
   GLX_GLOBAL float* residualOut = (GLX_GLOBAL float*)residualOut_ + tile.first * E;
   float y[U][E], r[U][E];
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    const uint32_t t = threadIdx.x + u * kBlock;
+    const uint32_t t = threadIdx.x + u * N;
     if (!FULL && t >= tile.lanes) continue;
     load<T, E, FULL>(x, t * E, tile.left, y[u]);
     if constexpr (RES_IN) load<F32, E, FULL>(residual, t * E, tile.left, r[u]);
   }
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    const uint32_t t = threadIdx.x + u * kBlock;
+    const uint32_t t = threadIdx.x + u * N;
     if (!FULL && t >= tile.lanes) continue;
     if constexpr (RES_IN) {
 #pragma unroll
@@ -254,7 +258,7 @@ __global__ __launch_bounds__(kBlock) void mx_quantize_kernel(char* payload,
                                                              float* residualOut, size_t n,
                                                              size_t nb, size_t tile0) {
   using Q = QuantizeShape<T, RES_IN || RES_OUT>;
-  const Tile<Q::E, Q::U> tile(tile0 + blockIdx.x, n, nb);
+  const Tile<Q::E, Q::U, kBlock> tile(tile0 + blockIdx.x, n, nb);
   if (tile.full) {
     quantize_tile<T, RES_IN, RES_OUT, true>(payload, x, residual, residualOut, nb, tile);
   } else {
@@ -273,11 +277,11 @@ template <int K, int E, bool NT>
 struct Part {
   typename Codes<E>::type code[K];
   uint8_t scale[K];
-  template <int U>
-  __device__ __forceinline__ void load(const MxSources& src, size_t nb, const Tile<E, U>& tile,
-                                       uint32_t t) {
+  template <int U, int N>
+  __device__ __forceinline__ void load(const MxSources& src, size_t nb,
+                                       const Tile<E, U, N>& tile, uint32_t t) {
     using C = typename Codes<E>::type;
-    constexpr uint32_t kLanes = Tile<E, U>::kLanes;
+    constexpr uint32_t kLanes = Tile<E, U, N>::kLanes;
 #pragma unroll
     for (int j = 0; j < K; j++) {
       const GLX_GLOBAL C* c = (const GLX_GLOBAL C*)src.p[j] + tile.first;
@@ -302,18 +306,18 @@ struct Part {
   }
 };
 
-template <typename T, int K, bool NT, bool FULL, int E, int U>
+template <typename T, int K, bool NT, bool FULL, int E, int U, int N>
 __device__ __forceinline__ void reduce_tile(typename T::S* dst, const MxSources& src, size_t nb,
-                                            float scale, const Tile<E, U>& tile) {
+                                            float scale, const Tile<E, U, N>& tile) {
   Part<K, E, NT> part[U];
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    const uint32_t t = threadIdx.x + u * kBlock;
+    const uint32_t t = threadIdx.x + u * N;
     if (FULL || t < tile.lanes) part[u].load(src, nb, tile, t);
   }
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    const uint32_t t = threadIdx.x + u * kBlock;
+    const uint32_t t = threadIdx.x + u * N;
     if (!FULL && t >= tile.lanes) continue;
     float acc[E];
     part[u].fold(scale, acc);
@@ -322,11 +326,12 @@ __device__ __forceinline__ void reduce_tile(typename T::S* dst, const MxSources&
 }
 
 template <typename T, int K, bool NT>
-__global__ __launch_bounds__(kBlock) void mx_reduce_n_kernel(typename T::S* dst, MxSources src,
-                                                             size_t n, size_t nb, float scale,
-                                                             size_t tile0) {
+__global__ __launch_bounds__(kReduceThreads) void mx_reduce_n_kernel(typename T::S* dst,
+                                                                     MxSources src, size_t n,
+                                                                     size_t nb, float scale,
+                                                                     size_t tile0) {
   constexpr int E = 16 / sizeof(typename T::S), U = kReduceParts<K>;
-  const Tile<E, U> tile(tile0 + blockIdx.x, n, nb);
+  const Tile<E, U, kReduceThreads> tile(tile0 + blockIdx.x, n, nb);
   if (tile.full) {
     reduce_tile<T, K, NT, true>(dst, src, nb, scale, tile);
   } else {
@@ -334,18 +339,18 @@ __global__ __launch_bounds__(kBlock) void mx_reduce_n_kernel(typename T::S* dst,
   }
 }
 
-template <int K, bool NT, bool FULL, int E, int U>
+template <int K, bool NT, bool FULL, int E, int U, int N>
 __device__ __forceinline__ void requantize_tile(char* payload, const MxSources& src, size_t nb,
-                                                float scale, const Tile<E, U>& tile) {
+                                                float scale, const Tile<E, U, N>& tile) {
   Part<K, E, NT> part[U];
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    const uint32_t t = threadIdx.x + u * kBlock;
+    const uint32_t t = threadIdx.x + u * N;
     if (FULL || t < tile.lanes) part[u].load(src, nb, tile, t);
   }
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    const uint32_t t = threadIdx.x + u * kBlock;
+    const uint32_t t = threadIdx.x + u * N;
     if (!FULL && t >= tile.lanes) continue;
     float acc[E];
     part[u].fold(scale, acc);
@@ -364,7 +369,7 @@ __global__ __launch_bounds__(kBlock) void mx_requantize_n_kernel(char* payload, 
                                                                  size_t n, size_t nb,
                                                                  float scale, size_t tile0) {
   constexpr int E = 8, U = kRequantizeParts<K>;
-  const Tile<E, U> tile(tile0 + blockIdx.x, n, nb);
+  const Tile<E, U, kBlock> tile(tile0 + blockIdx.x, n, nb);
   if (tile.full) {
     requantize_tile<K, NT, true>(payload, src, nb, scale, tile);
   } else {
@@ -378,8 +383,8 @@ __global__ __launch_bounds__(kBlock) void mx_requantize_n_kernel(char* payload, 
 constexpr size_t kTilesPerLaunch = size_t(1) << 20;
 
 template <typename Go>
-hipError_t over_tiles(size_t nb, int e, int u, Go go) {
-  const size_t per = (size_t)kBlock * u, tiles = (nb * (32 / e) + per - 1) / per;
+hipError_t over_tiles(size_t nb, int e, int u, int threads, Go go) {
+  const size_t per = (size_t)threads * u, tiles = (nb * (32 / e) + per - 1) / per;
   for (size_t at = 0; at < tiles; at += kTilesPerLaunch) {
     go(dim3((unsigned)std::min(tiles - at, kTilesPerLaunch)), at);
     const hipError_t err = hipGetLastError();
@@ -393,7 +398,7 @@ hipError_t quantize_with(void* payload, const void* x, const float* r, float* ro
                          hipStream_t s) {
   using Q = QuantizeShape<T, RES_IN || RES_OUT>;
   const size_t nb = mxBlocks(n);
-  return over_tiles(nb, Q::E, Q::U, [&](dim3 grid, size_t tile0) {
+  return over_tiles(nb, Q::E, Q::U, kBlock, [&](dim3 grid, size_t tile0) {
     hipLaunchKernelGGL((mx_quantize_kernel<T, RES_IN, RES_OUT>), grid, dim3(kBlock), 0, s,
                        (char*)payload, (const typename T::S*)x, r, ro, n, nb, tile0);
   });
@@ -427,12 +432,12 @@ hipError_t reduce_k(void* dst, const MxSources& src, size_t n, float scale, hipS
   constexpr int E = 16 / sizeof(typename T::S);
   const size_t nb = mxBlocks(n);
   const bool nt = streaming(src, K);
-  return over_tiles(nb, E, kReduceParts<K>, [&](dim3 grid, size_t tile0) {
+  return over_tiles(nb, E, kReduceParts<K>, kReduceThreads, [&](dim3 grid, size_t tile0) {
     if (K > 1 && nt) {
-      hipLaunchKernelGGL((mx_reduce_n_kernel<T, K, (K > 1)>), grid, dim3(kBlock), 0, s,
+      hipLaunchKernelGGL((mx_reduce_n_kernel<T, K, (K > 1)>), grid, dim3(kReduceThreads), 0, s,
                          (typename T::S*)dst, src, n, nb, scale, tile0);
     } else {
-      hipLaunchKernelGGL((mx_reduce_n_kernel<T, K, false>), grid, dim3(kBlock), 0, s,
+      hipLaunchKernelGGL((mx_reduce_n_kernel<T, K, false>), grid, dim3(kReduceThreads), 0, s,
                          (typename T::S*)dst, src, n, nb, scale, tile0);
     }
   });
@@ -443,7 +448,7 @@ hipError_t requantize_k(void* payload, const MxSources& src, size_t n, float sca
                         hipStream_t s) {
   const size_t nb = mxBlocks(n);
   const bool nt = streaming(src, K);
-  return over_tiles(nb, 8, kRequantizeParts<K>, [&](dim3 grid, size_t tile0) {
+  return over_tiles(nb, 8, kRequantizeParts<K>, kBlock, [&](dim3 grid, size_t tile0) {
     if (K > 1 && nt) {
       hipLaunchKernelGGL((mx_requantize_n_kernel<K, (K > 1)>), grid, dim3(kBlock), 0, s,
                          (char*)payload, src, n, nb, scale, tile0);

@@ -7,12 +7,15 @@ data-parallel program does with the buffers its allreduce returns.
 import ctypes
 
 from . import _lib
-from .algorithms import FLOAT32, FLOAT64, torch_dtype_code
+from .algorithms import BFLOAT16, FLOAT16, FLOAT32, FLOAT64
 from .errors import check, check_handle
 from .streams import as_torch_stream, current_stream_ptr
 
 lib = _lib.lib
 torch = _lib.torch
+_CODES = {} if torch is None else {
+    torch.float32: FLOAT32, torch.float64: FLOAT64, torch.float16: FLOAT16,
+    torch.bfloat16: BFLOAT16}
 
 
 def _dense(t):
@@ -25,6 +28,12 @@ def _dense(t):
             return False
         expect *= size
     return True
+
+
+def _same_order(a, b):
+    """Whether the strides of two tensors of one shape agree where they matter."""
+    return a.numel() == 0 or all(
+        x == y for x, y, n in zip(a.stride(), b.stride(), a.shape) if n > 1)
 
 
 class Gradients:
@@ -41,8 +50,9 @@ class Gradients:
     hipStream_t; default: torch's current stream) without synchronising, and
     can be captured in a HIP graph; each has a workspace of its own, so they
     may run at once on several streams.  The caller orders them after whatever
-    wrote the gradients, and keeps the object alive while its work, or a graph
-    holding it, runs."""
+    wrote the gradients, and keeps the object alive while a graph holding it is
+    replayed.  Make it outside of a capture, and once, not once a step: dropping
+    it waits for the device's work."""
 
     def __init__(self, grads, outs=None):
         grads = list(grads)
@@ -50,37 +60,36 @@ class Gradients:
         if outs is not None and len(outs) != len(grads):
             raise ValueError("%d gradients, %d outs" % (len(grads), len(outs)))
         self._h = None
+        device = grads[0].device if grads else None
         codes = []
         for i, t in enumerate(grads):
-            code = torch_dtype_code(t)
-            if not t.dtype.is_floating_point:
+            code = _CODES.get(t.dtype)
+            if code is None:
                 raise TypeError("gradient %d is %s" % (i, t.dtype))
             codes.append(code)
-            if not t.is_cuda or t.device != grads[0].device:
+            if not t.is_cuda or t.device != device:
                 raise ValueError("gradient %d is on %s" % (i, t.device))
             if t.is_neg():
                 raise ValueError("gradient %d is a negated view" % i)
-            if t.numel() and not _dense(t):
+            if not t.is_contiguous() and not _dense(t):
                 raise ValueError("gradient %d has gaps or overlaps in its memory (strides %s)"
-                                 % (i, tuple(t.stride())))
+                                 % (i, t.stride()))
             if outs is None:
                 continue
             o = outs[i]
-            if o.is_neg():
-                raise ValueError("out %d is a negated view" % i)
             if o.dtype != t.dtype:
                 raise TypeError("out %d is %s, its gradient %s" % (i, o.dtype, t.dtype))
-            if o.device != t.device or o.shape != t.shape or (
-                    t.numel() and any(a != b for a, b, s in zip(o.stride(), t.stride(), t.shape)
-                                      if s > 1)):
+            if o.is_neg():
+                raise ValueError("out %d is a negated view" % i)
+            if o.device != device or o.shape != t.shape or (
+                    o.stride() != t.stride() and not _same_order(o, t)):
                 raise ValueError("out %d does not have its gradient's device, shape and strides"
                                  % i)
         n = len(grads)
-        self.device = grads[0].device if grads else torch.device(
-            "cuda", torch.cuda.current_device())
-        self.dtype = torch.float64 if any(t.dtype == torch.float64 for t in grads) \
-            else torch.float32  # of the norm
-        self._code = FLOAT64 if self.dtype == torch.float64 else FLOAT32
+        self.device = device or torch.device("cuda", torch.cuda.current_device())
+        wide = FLOAT64 in codes
+        self.dtype = torch.float64 if wide else torch.float32  # of the norm
+        self._code = FLOAT64 if wide else FLOAT32
         # aliases hold the memory, also if a tensor is given another later
         self._keep = [t.detach() for t in grads] + [t.detach() for t in outs or ()]
         ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in grads])
@@ -145,7 +154,8 @@ class Gradients:
         return out
 
     def close(self):
-        """Free the handle (its work, and graphs holding it, must be done)."""
+        """Free the handle, after the work in flight on its device (no graph
+        holding it may be replayed afterwards)."""
         h, self._h = getattr(self, "_h", None), None
         if h:
             lib.glx_gradients_destroy(h)

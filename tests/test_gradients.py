@@ -476,6 +476,20 @@ def test_streams():
 
 
 @gpu
+def test_object_dropped_while_its_work_is_queued():
+    """Dropping the object waits for the device before its table goes."""
+    x = torch.ones(1 << 20, device="cuda")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(20_000_000)
+        n = Gradients([x]).norm()
+        fresh = [torch.full((64,), 255, dtype=torch.uint8, device="cuda") for _ in range(64)]
+    torch.cuda.synchronize()
+    assert float(n) == 1024 and len(fresh) == 64
+
+
+@gpu
 def test_two_streams_at_once():
     """One handle, two streams, many calls in flight: every result is right."""
     _, views = bucket([3000017, 5], torch.float32, 3, 1)
