@@ -380,7 +380,7 @@ __global__ __launch_bounds__(kBlock) void mx_requantize_n_kernel(char* payload, 
 
 // One workgroup per tile, so many tiles a launch: a grid has fewer than 2^32
 // threads.  go(grid, the launch's first tile).
-constexpr size_t kTilesPerLaunch = size_t(1) << 20;
+constexpr size_t kTilesPerLaunch = size_t(1) << 19;
 
 template <typename Go>
 hipError_t over_tiles(size_t nb, int e, int u, int threads, Go go) {

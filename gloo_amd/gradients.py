@@ -110,7 +110,7 @@ class Gradients:
         if self._h is None:
             raise ValueError("Gradients: closed")
         if out is None:
-            out = torch.empty((), dtype=dtype, device=self.device)
+            out = torch.empty_strided((), (), dtype=dtype, device=self.device)
         else:
             self._scalar(out, dtype, "out")
         ws = torch.empty(self._ws, dtype=torch.float64, device=self.device) if self._ws else None

@@ -518,6 +518,19 @@ def test_graph_replays():
         assert np.array_equal(eager.cpu().numpy(), payload_of(v.float().numpy())[0])
 
 
+def check_windows(x, y, spots, pay, out, n):
+    """Payload and values of x + residual = y in windows [at, at + m) that start
+    at blocks: y is a function of (at, m)."""
+    nb = -(-n // 32)
+    for at, m in spots:
+        exp, values = payload_of(y(at, m))
+        k = -(-m // 32)
+        assert np.array_equal(pay[at // 2:at // 2 + k * 16].cpu().numpy(), exp[:k * 16])
+        sc = nb * 16 + at // 32
+        assert np.array_equal(pay[sc:sc + k].cpu().numpy(), exp[k * 16:k * 17])
+        same_bits(as_numpy(out[at:at + m]), rounded(values.astype(np.float32), out.dtype))
+
+
 @gpu
 def test_offsets_beyond_32_bits():
     """2^32 + 77 elements: windows at the start, around 2^31 and 2^32, and the end."""
@@ -527,17 +540,35 @@ def test_offsets_beyond_32_bits():
     for i, (at, m) in enumerate(spots):
         x[at:at + m] = gradient(m, i, torch.bfloat16).cuda()
     pay = mx.quantize(x)
-    nb = -(-n // 32)
     out = torch.empty(n, dtype=torch.bfloat16, device="cuda")
     mx.dequantize(out, pay)
-    for at, m in spots:
-        exp, values = payload_of(x[at:at + m].float().cpu().numpy())
-        k = -(-m // 32)
-        assert np.array_equal(pay[at // 2:at // 2 + k * 16].cpu().numpy(), exp[:k * 16])
-        sc = nb * 16 + at // 32
-        assert np.array_equal(pay[sc:sc + k].cpu().numpy(), exp[k * 16:k * 17])
-        same_bits(as_numpy(out[at:at + m]), rounded(values.astype(np.float32), torch.bfloat16))
+    check_windows(x, lambda at, m: x[at:at + m].float().cpu().numpy(), spots, pay, out, n)
     assert int(out.count_nonzero()) <= sum(m for _, m in spots)
+    # the payload of a payload's values is that payload
+    again = torch.full_like(pay, 0xa5)
+    mx.requantize_n(again, [pay], n)
+    assert torch.equal(again, pay)
+
+
+@gpu
+def test_feedback_over_several_launches():
+    """float32 with feedback, longer than one launch takes (2^29 elements)."""
+    n = (1 << 29) + 1055
+    x = torch.zeros(n, device="cuda")
+    r = torch.zeros(n, device="cuda")
+    spots = [(0, 2048), ((1 << 29) - 1024, 2048 + 31)]
+    for i, (at, m) in enumerate(spots):
+        x[at:at + m] = gradient(m, i).cuda()
+        r[at:at + m] = gradient(m, 9 + i).cuda() * 0.1
+    left = torch.full_like(r, 7)
+    pay = mx.quantize(x, residual=r, residual_out=left)
+    out = torch.empty(n, device="cuda")
+    mx.dequantize(out, pay)
+
+    def y(at, m):
+        return (x[at:at + m] + r[at:at + m]).cpu().numpy()
+    check_windows(x, y, spots, pay, out, n)
+    assert torch.equal(left, (x + r) - out)
 
 
 # ---- with the rest of the framework ------------------------------------------
