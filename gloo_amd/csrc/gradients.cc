@@ -53,7 +53,10 @@ void checkOverlap(std::vector<Span>& spans) {
 
 int deviceOf(const void* p) {
   hipPointerAttribute_t a;
-  GLX_HIP_CHECK(hipPointerGetAttributes(&a, p));
+  if (hipPointerGetAttributes(&a, p) != hipSuccess) {
+    (void)hipGetLastError();  // not the next launch's error
+    a.type = hipMemoryTypeUnregistered;
+  }
   GLX_ENFORCE(a.type == hipMemoryTypeDevice, "not a device pointer");
   return a.device;
 }
@@ -127,9 +130,12 @@ GradientList::GradientList(const std::vector<void*>& grads, const std::vector<vo
   grid_ = (int)std::max<size_t>(1, std::min(table.size(), groups));
   if (nchunks_ > 0) {
     const size_t n = table.size() * sizeof(glx::GradChunk);
-    GLX_HIP_CHECK(hipMalloc((void**)&chunks_, n));
-    const hipError_t e = hipMemcpy(chunks_, table.data(), n, hipMemcpyHostToDevice);
-    if (e != hipSuccess) (void)hipFree(chunks_);
+    hipError_t e = hipMalloc((void**)&chunks_, n);
+    if (e == hipSuccess) {
+      e = hipMemcpy(chunks_, table.data(), n, hipMemcpyHostToDevice);
+      if (e != hipSuccess) (void)hipFree(chunks_);
+    }
+    if (e != hipSuccess) (void)hipGetLastError();  // not the next launch's error
     GLX_HIP_CHECK(e);
   }
 }
@@ -150,6 +156,7 @@ void GradientList::checkScalar(const void* p, int dtype, const char* what) const
                             [](const Span& s, uintptr_t e) { return s.at < e; });
   GLX_ENFORCE(i == spans_.begin() || (i - 1)->end <= at, "gradients: ", what,
               " lies in a tensor's memory");
+  deviceOf(p);
 }
 
 // The partials' memory, apart from the result.
@@ -160,6 +167,7 @@ void GradientList::checkWorkspace(const void* p, const void* scalar) const {
   const uintptr_t q = (uintptr_t)scalar;
   GLX_ENFORCE(scalar == nullptr || q < w || q >= end,
               "gradients: a scalar lies in the workspace");
+  deviceOf(p);
 }
 
 void GradientList::sum(int kind, bool root, int streamed, void* out, int outDtype,

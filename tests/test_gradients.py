@@ -411,6 +411,12 @@ def test_scalars_apart_from_the_tensors(n):
                                            None) == _lib.ERR_ENFORCE
     assert _lib.lib.glx_gradients_norm(g._h, 2.0, s.data_ptr(), 5 + 2, ws.data_ptr(), None) == \
         _lib.ERR_ENFORCE
+    host = np.zeros(1 << 14)
+    for call in (lambda: _lib.lib.glx_gradients_norm(g._h, 2.0, host.ctypes.data, 6,
+                                                     ws.data_ptr(), None),
+                 lambda: _lib.lib.glx_gradients_clip(g._h, 1.0, 2.0, host.ctypes.data, None, 0,
+                                                     None, None)):
+        assert call() == _lib.ERR_ENFORCE and "not a device pointer" in _lib.last_error()
     assert bool((x[1:-1] == 1).all())
     # no norm wanted: the clip alone
     assert _lib.lib.glx_gradients_clip(g._h, 0.5, float("inf"), None, None, 0, ws.data_ptr(),

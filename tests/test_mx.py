@@ -346,10 +346,19 @@ def test_quantize_refuses():
         mx.quantize(x, torch.zeros(64, dtype=torch.uint8, device="cuda")[8:56])
     with pytest.raises(gloo_amd.EnforceNotMet, match="shares"):
         mx.quantize(x, x.view(torch.uint8)[:48])
-    with pytest.raises(gloo_amd.EnforceNotMet, match="not a device pointer"):
-        host = np.zeros(64, np.uint8)
-        at = host.ctypes.data + -host.ctypes.data % 16
-        gloo_amd.errors.check(_lib.lib.glx_mx_quantize(5, at, x.data_ptr(), None, None, 4, None))
+    host = np.zeros(4096, np.uint8)
+    at = host.ctypes.data + -host.ctypes.data % 16
+    L, xp, pp = _lib.lib, x.data_ptr(), p.data_ptr()
+    for call in (lambda: L.glx_mx_quantize(5, at, xp, None, None, 4, None),
+                 lambda: L.glx_mx_quantize(5, pp, at, None, None, 4, None),
+                 lambda: L.glx_mx_quantize(5, pp, xp, at, None, 4, None),
+                 lambda: L.glx_mx_quantize(5, pp, xp, None, at, 4, None),
+                 lambda: L.glx_mx_reduce_n(5, at, P16(pp), 1, 4, 1.0, None),
+                 lambda: L.glx_mx_reduce_n(5, xp, P16(pp, at), 2, 4, 1.0, None),
+                 lambda: L.glx_mx_requantize_n(at, P16(pp), 1, 4, 1.0, None),
+                 lambda: L.glx_mx_requantize_n(pp, P16(at), 1, 4, 1.0, None)):
+        with pytest.raises(gloo_amd.EnforceNotMet, match="not a device pointer"):
+            gloo_amd.errors.check(call())
 
 
 # ---- the fold ----------------------------------------------------------------
