@@ -167,7 +167,6 @@ void GradientList::checkWorkspace(const void* p, const void* scalar) const {
   const uintptr_t q = (uintptr_t)scalar;
   GLX_ENFORCE(scalar == nullptr || q < w || q >= end,
               "gradients: a scalar lies in the workspace");
-  deviceOf(p);
 }
 
 void GradientList::sum(int kind, bool root, int streamed, void* out, int outDtype,

@@ -51,11 +51,14 @@ def _code(t, what):
     return code
 
 
-def _payload_ptr(t, need, device, what="payload"):
-    _check(t, what, device)
-    if t.dtype != torch.uint8:
-        raise TypeError("mx: %s is %s, not uint8" % (what, t.dtype))
-    if t.numel() < need:
+def _payload_ptr(t, need, device, j=None):
+    """Address of a payload (the j-th source) of at least `need` bytes."""
+    if t.dtype != torch.uint8 or t.device != device or not t.is_contiguous() or t.is_neg() or \
+            t.numel() < need or not t.is_cuda:
+        what = "payload" if j is None else "payload %d" % j
+        _check(t, what, device)
+        if t.dtype != torch.uint8:
+            raise TypeError("mx: %s is %s, not uint8" % (what, t.dtype))
         raise ValueError("mx: %s has %d bytes of the %d needed" % (what, t.numel(), need))
     return t.data_ptr()
 
@@ -92,7 +95,7 @@ def quantize(x, payload=None, residual=None, residual_out=None, stream=None):
 
 
 def _sources(payloads, need, device):
-    ptrs = [_payload_ptr(t, need, device, "payload %d" % j) for j, t in enumerate(payloads)]
+    ptrs = [_payload_ptr(t, need, device, j) for j, t in enumerate(payloads)]
     return (ctypes.c_void_p * len(ptrs))(*ptrs), len(ptrs)
 
 
