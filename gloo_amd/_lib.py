@@ -136,6 +136,9 @@ SIGNATURES = [
     ("glx_mx_quantize", _i, [_i, _vp, _vp, _vp, _vp, _sz, _vp]),
     ("glx_mx_reduce_n", _i, [_i, _vp, ctypes.POINTER(_vp), _i, _sz, ctypes.c_float, _vp]),
     ("glx_mx_requantize_n", _i, [_vp, ctypes.POINTER(_vp), _i, _sz, ctypes.c_float, _vp]),
+    ("glx_mx_quantize_on", _i, [_i, _i, _vp, _vp, _vp, _vp, _sz, _vp]),
+    ("glx_mx_reduce_n_on", _i, [_i, _i, _vp, ctypes.POINTER(_vp), _i, _sz, ctypes.c_float, _vp]),
+    ("glx_mx_requantize_n_on", _i, [_i, _vp, ctypes.POINTER(_vp), _i, _sz, ctypes.c_float, _vp]),
 ]
 
 for _name, _res, _args in SIGNATURES:

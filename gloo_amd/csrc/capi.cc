@@ -124,8 +124,6 @@ bool overlaps(const void* a, size_t na, const void* b, size_t nb) {
   return a != nullptr && b != nullptr && x < y + nb && y < x + na;
 }
 
-// What is read is not looked up (0.3 us a pointer): only where the result goes,
-// which tells the device.
 void checkMxPayloads(const void* const* payloads, int k) {
   GLX_ENFORCE(payloads != nullptr && k >= 1 && k <= glx::kMxMaxSources,
               "mx: need 1..", glx::kMxMaxSources, " payloads");
@@ -133,6 +131,98 @@ void checkMxPayloads(const void* const* payloads, int k) {
     GLX_ENFORCE(payloads[j] != nullptr && (uintptr_t)payloads[j] % 16 == 0, "mx: payload ", j,
                 " is null or not 16-byte aligned");
   }
+}
+
+// Where a message operator runs: on `device`, if the caller states it, or on
+// that of `result`.  Then nothing is known of the other pointers either, and host
+// memory that is not pinned would end the process in the kernel: each is looked up
+// (0.3 us).
+constexpr int kLookUp = -1;
+int mxDevice(int device, const void* result) {
+  return device == kLookUp ? gloo::deviceOf(result) : device;
+}
+void checkMxReach(int device, const void* p, const char* what) {
+  if (device != kLookUp || p == nullptr) return;
+  GLX_ENFORCE(gloo::reachable(p), "mx: ", what, " is host memory that no device reaches");
+}
+void checkMxReach(int device, const void* const* payloads, int k) {
+  for (int j = 0; device == kLookUp && j < k; j++) {
+    GLX_ENFORCE(gloo::reachable(payloads[j]), "mx: payload ", j,
+                " is host memory that no device reaches");
+  }
+}
+
+int mxQuantize(int device, int dtype, void* payload, const void* x, const float* residual,
+               float* residual_out, size_t n, glx_stream_t stream) {
+  GLX_ENFORCE(mxDtype(dtype), "glx_mx_quantize: float32, float16 or bfloat16");
+  GLX_ENFORCE(n <= (size_t(1) << 60), "glx_mx_quantize: too many elements");
+  if (n == 0) return GLX_OK;
+  const size_t es = glx_dtype_size(dtype), bytes = glx::mxPayloadBytes(n);
+  checkMxPayloads(&payload, 1);
+  GLX_ENFORCE(x != nullptr && (uintptr_t)x % es == 0, "glx_mx_quantize: null or misaligned x");
+  GLX_ENFORCE((uintptr_t)residual % 4 == 0 && (uintptr_t)residual_out % 4 == 0,
+              "glx_mx_quantize: misaligned residual");
+  GLX_ENFORCE(!overlaps(payload, bytes, x, n * es) &&
+                  !overlaps(payload, bytes, residual, n * 4) &&
+                  !overlaps(payload, bytes, residual_out, n * 4),
+              "glx_mx_quantize: the payload shares memory with another buffer");
+  GLX_ENFORCE(residual_out == residual || !overlaps(residual_out, n * 4, residual, n * 4),
+              "glx_mx_quantize: the residuals overlap");
+  GLX_ENFORCE((const void*)residual_out == x ? dtype == GLX_FLOAT32
+                                             : !overlaps(residual_out, n * 4, x, n * es),
+              "glx_mx_quantize: residual_out overlaps x");
+  checkMxReach(device, x, "x");
+  checkMxReach(device, residual, "residual");
+  checkMxReach(device, residual_out, "residual_out");
+  gloo::DeviceScope scope(mxDevice(device, payload));
+  return hipStatus(glx::launch_mx_quantize(dtype, payload, x, residual, residual_out, n,
+                                           (hipStream_t)stream),
+                   "glx_mx_quantize");
+}
+
+int mxReduceN(int device, int dtype, void* dst, const void* const* payloads, int k, size_t n,
+              float scale, glx_stream_t stream) {
+  GLX_ENFORCE(mxDtype(dtype), "glx_mx_reduce_n: float32, float16 or bfloat16");
+  GLX_ENFORCE(n <= (size_t(1) << 60), "glx_mx_reduce_n: too many elements");
+  GLX_ENFORCE(std::isfinite(scale), "glx_mx_reduce_n: scale is not finite");
+  if (n == 0) return GLX_OK;
+  const size_t es = glx_dtype_size(dtype), bytes = glx::mxPayloadBytes(n);
+  checkMxPayloads(payloads, k);
+  GLX_ENFORCE(dst != nullptr && (uintptr_t)dst % es == 0,
+              "glx_mx_reduce_n: null or misaligned dst");
+  for (int j = 0; j < k; j++) {
+    GLX_ENFORCE(!overlaps(dst, n * es, payloads[j], bytes), "glx_mx_reduce_n: dst and payload ",
+                j, " share memory");
+  }
+  checkMxReach(device, payloads, k);
+  gloo::DeviceScope scope(mxDevice(device, dst));
+  return hipStatus(
+      glx::launch_mx_reduce_n(dtype, dst, payloads, k, n, scale, (hipStream_t)stream),
+      "glx_mx_reduce_n");
+}
+
+int mxRequantizeN(int device, void* payload, const void* const* payloads, int k, size_t n,
+                  float scale, glx_stream_t stream) {
+  GLX_ENFORCE(n <= (size_t(1) << 60), "glx_mx_requantize_n: too many elements");
+  GLX_ENFORCE(std::isfinite(scale), "glx_mx_requantize_n: scale is not finite");
+  if (n == 0) return GLX_OK;
+  const size_t bytes = glx::mxPayloadBytes(n);
+  checkMxPayloads(payloads, k);
+  checkMxPayloads(&payload, 1);
+  for (int j = 0; j < k; j++) {
+    GLX_ENFORCE(payload == payloads[j] || !overlaps(payload, bytes, payloads[j], bytes),
+                "glx_mx_requantize_n: the payload overlaps source ", j);
+  }
+  checkMxReach(device, payloads, k);
+  gloo::DeviceScope scope(mxDevice(device, payload));
+  return hipStatus(
+      glx::launch_mx_requantize_n(payload, payloads, k, n, scale, (hipStream_t)stream),
+      "glx_mx_requantize_n");
+}
+
+int statedDevice(int device, const char* what) {
+  GLX_ENFORCE(device >= 0, what, ": negative device");
+  return device;
 }
 
 }  // namespace
@@ -1064,70 +1154,45 @@ size_t glx_mx_payload_bytes(size_t n) { return glx::mxPayloadBytes(n); }
 
 int glx_mx_quantize(int dtype, void* payload, const void* x, const float* residual,
                     float* residual_out, size_t n, glx_stream_t stream) {
-  return guarded([&]() -> int {
-    GLX_ENFORCE(mxDtype(dtype), "glx_mx_quantize: float32, float16 or bfloat16");
-    GLX_ENFORCE(n <= (size_t(1) << 60), "glx_mx_quantize: too many elements");
-    if (n == 0) return GLX_OK;
-    const size_t es = glx_dtype_size(dtype), bytes = glx::mxPayloadBytes(n);
-    checkMxPayloads(&payload, 1);
-    GLX_ENFORCE(x != nullptr && (uintptr_t)x % es == 0, "glx_mx_quantize: null or misaligned x");
-    GLX_ENFORCE((uintptr_t)residual % 4 == 0 && (uintptr_t)residual_out % 4 == 0,
-                "glx_mx_quantize: misaligned residual");
-    GLX_ENFORCE(!overlaps(payload, bytes, x, n * es) &&
-                    !overlaps(payload, bytes, residual, n * 4) &&
-                    !overlaps(payload, bytes, residual_out, n * 4),
-                "glx_mx_quantize: the payload shares memory with another buffer");
-    GLX_ENFORCE(residual_out == residual || !overlaps(residual_out, n * 4, residual, n * 4),
-                "glx_mx_quantize: the residuals overlap");
-    GLX_ENFORCE((const void*)residual_out == x ? dtype == GLX_FLOAT32
-                                               : !overlaps(residual_out, n * 4, x, n * es),
-                "glx_mx_quantize: residual_out overlaps x");
-    gloo::DeviceScope scope(gloo::deviceOf(payload));
-    return hipStatus(glx::launch_mx_quantize(dtype, payload, x, residual, residual_out, n,
-                                             (hipStream_t)stream),
-                     "glx_mx_quantize");
+  return guarded([&] {
+    return mxQuantize(kLookUp, dtype, payload, x, residual, residual_out, n, stream);
+  });
+}
+
+int glx_mx_quantize_on(int device, int dtype, void* payload, const void* x,
+                       const float* residual, float* residual_out, size_t n,
+                       glx_stream_t stream) {
+  return guarded([&] {
+    return mxQuantize(statedDevice(device, "glx_mx_quantize_on"), dtype, payload, x, residual,
+                      residual_out, n, stream);
   });
 }
 
 int glx_mx_reduce_n(int dtype, void* dst, const void* const* payloads, int k, size_t n,
                     float scale, glx_stream_t stream) {
-  return guarded([&]() -> int {
-    GLX_ENFORCE(mxDtype(dtype), "glx_mx_reduce_n: float32, float16 or bfloat16");
-    GLX_ENFORCE(n <= (size_t(1) << 60), "glx_mx_reduce_n: too many elements");
-    GLX_ENFORCE(std::isfinite(scale), "glx_mx_reduce_n: scale is not finite");
-    if (n == 0) return GLX_OK;
-    const size_t es = glx_dtype_size(dtype), bytes = glx::mxPayloadBytes(n);
-    checkMxPayloads(payloads, k);
-    GLX_ENFORCE(dst != nullptr && (uintptr_t)dst % es == 0,
-                "glx_mx_reduce_n: null or misaligned dst");
-    for (int j = 0; j < k; j++) {
-      GLX_ENFORCE(!overlaps(dst, n * es, payloads[j], bytes), "glx_mx_reduce_n: dst and payload ",
-                  j, " share memory");
-    }
-    gloo::DeviceScope scope(gloo::deviceOf(dst));
-    return hipStatus(
-        glx::launch_mx_reduce_n(dtype, dst, payloads, k, n, scale, (hipStream_t)stream),
-        "glx_mx_reduce_n");
+  return guarded(
+      [&] { return mxReduceN(kLookUp, dtype, dst, payloads, k, n, scale, stream); });
+}
+
+int glx_mx_reduce_n_on(int device, int dtype, void* dst, const void* const* payloads, int k,
+                       size_t n, float scale, glx_stream_t stream) {
+  return guarded([&] {
+    return mxReduceN(statedDevice(device, "glx_mx_reduce_n_on"), dtype, dst, payloads, k, n,
+                     scale, stream);
   });
 }
 
 int glx_mx_requantize_n(void* payload, const void* const* payloads, int k, size_t n,
                         float scale, glx_stream_t stream) {
-  return guarded([&]() -> int {
-    GLX_ENFORCE(n <= (size_t(1) << 60), "glx_mx_requantize_n: too many elements");
-    GLX_ENFORCE(std::isfinite(scale), "glx_mx_requantize_n: scale is not finite");
-    if (n == 0) return GLX_OK;
-    const size_t bytes = glx::mxPayloadBytes(n);
-    checkMxPayloads(payloads, k);
-    checkMxPayloads(&payload, 1);
-    for (int j = 0; j < k; j++) {
-      GLX_ENFORCE(payload == payloads[j] || !overlaps(payload, bytes, payloads[j], bytes),
-                  "glx_mx_requantize_n: the payload overlaps source ", j);
-    }
-    gloo::DeviceScope scope(gloo::deviceOf(payload));
-    return hipStatus(
-        glx::launch_mx_requantize_n(payload, payloads, k, n, scale, (hipStream_t)stream),
-        "glx_mx_requantize_n");
+  return guarded(
+      [&] { return mxRequantizeN(kLookUp, payload, payloads, k, n, scale, stream); });
+}
+
+int glx_mx_requantize_n_on(int device, void* payload, const void* const* payloads, int k,
+                           size_t n, float scale, glx_stream_t stream) {
+  return guarded([&] {
+    return mxRequantizeN(statedDevice(device, "glx_mx_requantize_n_on"), payload, payloads, k, n,
+                         scale, stream);
   });
 }
 

@@ -51,15 +51,26 @@ void checkOverlap(std::vector<Span>& spans) {
 
 }  // namespace
 
-int deviceOf(const void* p) {
+namespace {
+
+hipPointerAttribute_t attributesOf(const void* p) {
   hipPointerAttribute_t a;
   if (hipPointerGetAttributes(&a, p) != hipSuccess) {
     (void)hipGetLastError();  // not the next launch's error
     a.type = hipMemoryTypeUnregistered;
   }
+  return a;
+}
+
+}  // namespace
+
+int deviceOf(const void* p) {
+  const hipPointerAttribute_t a = attributesOf(p);
   GLX_ENFORCE(a.type == hipMemoryTypeDevice, "not a device pointer");
   return a.device;
 }
+
+bool reachable(const void* p) { return attributesOf(p).type != hipMemoryTypeUnregistered; }
 
 DeviceScope::DeviceScope(int device) {
   int cur = -1;

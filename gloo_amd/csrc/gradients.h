@@ -64,6 +64,9 @@ class DeviceScope {
 // The device whose memory p is in (EnforceNotMet: not device memory).
 int deviceOf(const void* p);
 
+// Whether kernels can reach p: memory of a device, or host memory pinned for it.
+bool reachable(const void* p);
+
 // A list of gradient tensors on one device, laid out once into a table of
 // chunks in device memory.  Read-only afterwards: any number of calls may run
 // at once, each with a workspace of its own.

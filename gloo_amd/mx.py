@@ -87,10 +87,10 @@ def quantize(x, payload=None, residual=None, residual_out=None, stream=None):
     need = payload_bytes(n)
     if payload is None:
         payload = torch.empty(need, dtype=torch.uint8, device=device)
-    check(lib.glx_mx_quantize(code, _payload_ptr(payload, need, device), x.data_ptr(),
-                              _residual_ptr(residual, n, device, "residual"),
-                              _residual_ptr(residual_out, n, device, "residual_out"),
-                              n, current_stream_ptr(device)), "mx.quantize")
+    check(lib.glx_mx_quantize_on(device.index, code, _payload_ptr(payload, need, device),
+                                 x.data_ptr(), _residual_ptr(residual, n, device, "residual"),
+                                 _residual_ptr(residual_out, n, device, "residual_out"),
+                                 n, current_stream_ptr(device)), "mx.quantize")
     return payload
 
 
@@ -108,8 +108,8 @@ def reduce_n(dst, payloads, scale=1.0, stream=None):
     _check(dst, "dst")
     code, n, device = _code(dst, "dst"), dst.numel(), dst.device
     arr, k = _sources(payloads, payload_bytes(n), device)
-    check(lib.glx_mx_reduce_n(code, dst.data_ptr(), arr, k, n, scale,
-                              current_stream_ptr(device)), "mx.reduce_n")
+    check(lib.glx_mx_reduce_n_on(device.index, code, dst.data_ptr(), arr, k, n, scale,
+                                 current_stream_ptr(device)), "mx.reduce_n")
     return dst
 
 
@@ -128,6 +128,6 @@ def requantize_n(payload, payloads, n, scale=1.0, stream=None):
     need, device = payload_bytes(n), payload.device
     out = _payload_ptr(payload, need, device)
     arr, k = _sources(payloads, need, device)
-    check(lib.glx_mx_requantize_n(out, arr, k, n, scale, current_stream_ptr(device)),
-          "mx.requantize_n")
+    check(lib.glx_mx_requantize_n_on(device.index, out, arr, k, n, scale,
+                                     current_stream_ptr(device)), "mx.requantize_n")
     return payload

@@ -1,0 +1,246 @@
+// gradients_host_test.cc -- what glx_mx_* and glx_gradients_* decide on the
+// host, on two imagined GPUs: the HIP functions that these calls use are defined
+// here, and an executable's definitions come before the runtime's, so every
+// launch is written down and none happens.  Needs no GPU.
+//   gradients_host_test CASE     exit status 0 = passed
+#include <hip/hip_runtime_api.h>
+
+#include <cstdio>
+#include <cstring>
+#include <map>
+#include <string>
+#include <vector>
+
+#include "gloo_amd/glx.h"
+
+namespace {
+
+int g_failures = 0;
+
+#define EXPECT(cond)                                                       \
+  do {                                                                     \
+    if (!(cond)) {                                                         \
+      std::fprintf(stderr, "FAIL %s:%d: %s\n", __FILE__, __LINE__, #cond); \
+      g_failures++;                                                        \
+    }                                                                      \
+  } while (0)
+
+// ---- the imagined machine ---------------------------------------------------
+
+// Addresses: a stretch of memory per GPU, one of pinned host memory; all others
+// are pageable host memory.
+constexpr uintptr_t kStretch = uintptr_t(1) << 44;
+constexpr int kDevices = 2;
+char* device(int d, size_t at) { return (char*)(kStretch * (d + 1) + at); }
+char* pinned(size_t at) { return (char*)(kStretch * (kDevices + 1) + at); }
+char* pageable(size_t at) { return (char*)(kStretch * (kDevices + 2) + at); }
+
+struct Launch {
+  std::string kernel;
+  int device;
+  hipStream_t stream;
+  void** args;  // valid during the launch only
+};
+struct Machine {
+  int current = 0, lookups = 0, frees = 0;
+  size_t next = kStretch / 2;  // of hipMalloc
+  hipError_t error = hipSuccess;
+  std::vector<Launch> launches;
+  void (*onLaunch)(const Launch&) = nullptr;
+};
+Machine m;
+
+std::map<const void*, std::string>& kernels() {  // filled before main()
+  static std::map<const void*, std::string> k;
+  return k;
+}
+
+hipError_t left(hipError_t e) {
+  if (e != hipSuccess) m.error = e;
+  return e;
+}
+
+}  // namespace
+
+extern "C" {
+
+hipError_t hipGetLastError() {
+  const hipError_t e = m.error;
+  m.error = hipSuccess;
+  return e;
+}
+hipError_t hipGetDevice(int* d) {
+  *d = m.current;
+  return hipSuccess;
+}
+hipError_t hipSetDevice(int d) {
+  if (d < 0 || d >= kDevices) return left(hipErrorInvalidDevice);
+  m.current = d;
+  return hipSuccess;
+}
+hipError_t hipDeviceGetAttribute(int* v, hipDeviceAttribute_t, int) {
+  *v = 256;
+  return hipSuccess;
+}
+hipError_t hipPointerGetAttributes(hipPointerAttribute_t* a, const void* p) {
+  m.lookups++;
+  std::memset(a, 0, sizeof(*a));
+  const uintptr_t s = (uintptr_t)p / kStretch;
+  if (s < 1 || s > kDevices + 1) return left(hipErrorInvalidValue);
+  a->type = s <= kDevices ? hipMemoryTypeDevice : hipMemoryTypeHost;
+  a->device = s <= kDevices ? (int)s - 1 : 0;
+  a->devicePointer = (void*)p;
+  return hipSuccess;
+}
+hipError_t hipMalloc(void** p, size_t n) {
+  *p = device(m.current, m.next);
+  m.next += (n + 4095) / 4096 * 4096;
+  return hipSuccess;
+}
+hipError_t hipMemcpy(void*, const void*, size_t, hipMemcpyKind) { return hipSuccess; }
+hipError_t hipFree(void*) {
+  m.frees++;
+  return hipSuccess;
+}
+void __hipRegisterFunction(void**, const void* host, char*, const char* name, unsigned, void*,
+                           void*, void*, void*, int*) {
+  kernels()[host] = name;
+}
+namespace {
+dim3 g_grid, g_block;
+size_t g_shared;
+hipStream_t g_stream;
+}
+hipError_t __hipPushCallConfiguration(dim3 grid, dim3 block, size_t shared, hipStream_t s) {
+  g_grid = grid, g_block = block, g_shared = shared, g_stream = s;
+  return hipSuccess;
+}
+hipError_t __hipPopCallConfiguration(dim3* grid, dim3* block, size_t* shared, hipStream_t* s) {
+  *grid = g_grid, *block = g_block, *shared = g_shared, *s = g_stream;
+  return hipSuccess;
+}
+hipError_t hipLaunchKernel(const void* f, dim3, dim3, void** args, size_t, hipStream_t s) {
+  m.launches.push_back({kernels()[f], m.current, s, args});
+  if (m.onLaunch != nullptr) m.onLaunch(m.launches.back());
+  return hipSuccess;
+}
+
+}  // extern "C"
+
+namespace {
+
+const glx_stream_t kStream = (glx_stream_t)0x1234;
+
+// A refusal: its message, nothing launched, the device as it was, and no error
+// that the next HIP call would be taken to have made.
+void refused(int line, int status, const char* message) {
+  const bool ok = status == GLX_ERR_ENFORCE && std::strstr(glx_last_error(), message) != nullptr &&
+                  m.launches.empty() && m.current == 0 && m.error == hipSuccess;
+  if (!ok) {
+    std::fprintf(stderr, "FAIL line %d: status %d, \"%s\" for \"%s\", %zu launches\n", line, status,
+                 glx_last_error(), message, m.launches.size());
+    g_failures++;
+  }
+  m.launches.clear();
+  m.error = hipSuccess;
+}
+#define REFUSED(call, message) refused(__LINE__, call, message)
+
+// One launch of a kernel on a device, and the current device back.
+void launched(int line, int status, const char* kernel, int dev) {
+  const bool ok = status == GLX_OK && m.launches.size() == 1 &&
+                  m.launches[0].kernel.find(kernel) != std::string::npos &&
+                  m.launches[0].device == dev && m.launches[0].stream == kStream && m.current == 0;
+  if (!ok) {
+    std::fprintf(stderr, "FAIL line %d: status %d \"%s\", %zu launches, the first %s on %d\n", line,
+                 status, glx_last_error(), m.launches.size(),
+                 m.launches.empty() ? "-" : m.launches[0].kernel.c_str(),
+                 m.launches.empty() ? -1 : m.launches[0].device);
+    g_failures++;
+  }
+  m.launches.clear();
+}
+#define LAUNCHED(call, kernel, dev) launched(__LINE__, call, kernel, dev)
+
+// ---- cases ------------------------------------------------------------------
+
+constexpr size_t kN = 4099, kMiB = 1 << 20;
+
+void mxPointers() {
+  const int f32 = GLX_FLOAT32;
+  char *pay = device(0, 0), *x = device(0, kMiB), *r = device(0, 2 * kMiB), *host = pageable(0);
+  float *ro = (float*)device(0, 3 * kMiB), *rf = (float*)r;
+  auto quantize = [&](void* payload, void* src, void* res, float* out) {
+    return glx_mx_quantize(f32, payload, src, (float*)res, out, kN, kStream);
+  };
+  REFUSED(quantize(host, x, r, ro), "not a device pointer");
+  REFUSED(quantize(pay, host, r, ro), "x is");
+  REFUSED(quantize(pay, x, host, ro), "residual is");
+  REFUSED(quantize(pay, x, r, (float*)host), "residual_out is");
+  REFUSED(quantize(pay, host, nullptr, nullptr), "x is");
+  LAUNCHED(quantize(pay, x, r, ro), "quantize", 0);
+  LAUNCHED(quantize(pay, x, r, rf), "quantize", 0);
+  LAUNCHED(quantize(pay, x, nullptr, nullptr), "quantize", 0);
+  // what a kernel reaches may be pinned host memory
+  LAUNCHED(quantize(pay, pinned(0), r, (float*)pinned(kMiB)), "quantize", 0);
+  LAUNCHED(quantize(device(1, 0), device(1, kMiB), nullptr, nullptr), "quantize", 1);
+
+  for (int k = 1; k <= 16; k++) {
+    std::vector<const void*> src;
+    for (int j = 0; j < k; j++) src.push_back(device(0, (4 + j) * kMiB));
+    auto reduce = [&](void* dst) {
+      return glx_mx_reduce_n(f32, dst, src.data(), k, kN, 0.5f, kStream);
+    };
+    auto requantize = [&](void* to) {
+      return glx_mx_requantize_n(to, src.data(), k, kN, 0.5f, kStream);
+    };
+    LAUNCHED(reduce(x), "reduce_n", 0);
+    LAUNCHED(requantize(pay), "requantize_n", 0);
+    LAUNCHED(requantize((void*)src[0]), "requantize_n", 0);
+    REFUSED(reduce(host), "not a device pointer");
+    REFUSED(requantize(host), "not a device pointer");
+    for (int j = 0; j < k; j++) {
+      const void* was = src[j];
+      src[j] = host;
+      const std::string name = "payload " + std::to_string(j) + " is";
+      REFUSED(reduce(x), name.c_str());
+      REFUSED(requantize(pay), name.c_str());
+      src[j] = pinned(0);
+      LAUNCHED(reduce(x), "reduce_n", 0);
+      src[j] = was;
+    }
+  }
+}
+
+// The calls on a stated device look nothing up.
+void mxOn() {
+  const void* src[2] = {device(1, kMiB), device(1, 2 * kMiB)};
+  m.lookups = 0;
+  LAUNCHED(glx_mx_quantize_on(1, GLX_FLOAT32, device(1, 0), device(1, kMiB), nullptr, nullptr, kN,
+                              kStream),
+           "quantize", 1);
+  LAUNCHED(glx_mx_reduce_n_on(1, GLX_BFLOAT16, device(1, 0), src, 2, kN, 1, kStream), "reduce_n",
+           1);
+  LAUNCHED(glx_mx_requantize_n_on(1, device(1, 0), src, 2, kN, 1, kStream), "requantize_n", 1);
+  EXPECT(m.lookups == 0);
+  REFUSED(glx_mx_reduce_n_on(-1, GLX_FLOAT32, device(1, 0), src, 2, kN, 1, kStream), "negative");
+  REFUSED(glx_mx_requantize_n_on(1, device(1, kMiB + 16), src, 2, kN, 1, kStream), "overlaps");
+  EXPECT(glx_mx_reduce_n_on(kDevices, GLX_FLOAT32, device(1, 0), src, 2, kN, 1, kStream) ==
+         GLX_ERR_HIP);
+  EXPECT(m.launches.empty() && m.current == 0);
+}
+
+const std::map<std::string, void (*)()> kCases = {
+    {"mx_pointers", mxPointers},
+    {"mx_on", mxOn},
+};
+
+}  // namespace
+
+int main(int argc, char** argv) {
+  const auto c = argc == 2 ? kCases.find(argv[1]) : kCases.end();
+  if (c == kCases.end()) return 2;
+  c->second();
+  if (g_failures == 0) std::printf("passed\n");
+  return g_failures == 0 ? 0 : 1;
+}

@@ -356,6 +356,39 @@ def test_quantize_refuses():
             gloo_amd.errors.check(call())
 
 
+@gpu
+def test_host_memory_is_refused_at_every_pointer():
+    """By the C ABI, on the host: nothing is launched.  Pinned memory is not host
+    memory in this sense, kernels reach it."""
+    x = gradient(64, 3).cuda()
+    p = torch.full((48,), 0xa5, dtype=torch.uint8, device="cuda")
+    r = torch.zeros(64, device="cuda")
+    host = np.zeros(4096, np.uint8)
+    at = host.ctypes.data + -host.ctypes.data % 16
+    L, xp, pp, rp = _lib.lib, x.data_ptr(), p.data_ptr(), r.data_ptr()
+    for call, what in (
+            (lambda: L.glx_mx_quantize(5, at, xp, rp, rp, 64, None), "device pointer"),
+            (lambda: L.glx_mx_quantize(5, pp, at, rp, rp, 64, None), "x is host"),
+            (lambda: L.glx_mx_quantize(5, pp, xp, at, rp, 64, None), "residual is host"),
+            (lambda: L.glx_mx_quantize(5, pp, xp, rp, at, 64, None), "residual_out is host"),
+            (lambda: L.glx_mx_reduce_n(5, at, P16(pp), 1, 64, 1.0, None), "device pointer"),
+            (lambda: L.glx_mx_reduce_n(5, xp, P16(pp, at), 2, 64, 1.0, None), "payload 1 is host"),
+            (lambda: L.glx_mx_requantize_n(at, P16(pp), 1, 64, 1.0, None), "device pointer"),
+            (lambda: L.glx_mx_requantize_n(pp, P16(at), 1, 64, 1.0, None), "payload 0 is host")):
+        with pytest.raises(gloo_amd.EnforceNotMet, match=what):
+            gloo_amd.errors.check(call())
+    torch.cuda.synchronize()
+    assert bool((p == 0xa5).all()) and not bool(r.any()) and not host.any()
+    exp, values = payload_of(x.cpu().numpy())
+    px = torch.empty(64, pin_memory=True).copy_(x)
+    pr = torch.full((64,), 7.0, pin_memory=True)
+    torch.cuda.synchronize()
+    gloo_amd.errors.check(L.glx_mx_quantize(5, pp, px.data_ptr(), None, pr.data_ptr(), 64, None))
+    torch.cuda.synchronize()
+    assert np.array_equal(p.cpu().numpy(), exp)
+    assert np.array_equal(pr.numpy().astype(np.float64), x.cpu().numpy() - values)
+
+
 # ---- the fold ----------------------------------------------------------------
 
 @gpu
