@@ -155,29 +155,37 @@ GradientList::~GradientList() {
   if (chunks_ != nullptr) (void)hipFree(chunks_);
 }
 
+// Memory of a call outside the tensors, which other workgroups read and write.
+void GradientList::checkApart(const void* p, size_t bytes, const char* what) const {
+  const uintptr_t at = (uintptr_t)p, end = at + bytes;
+  // spans_ is sorted and without overlap: only the last one that begins before
+  // the end can reach it
+  auto i = std::lower_bound(spans_.begin(), spans_.end(), end,
+                            [](const Span& s, uintptr_t e) { return s.at < e; });
+  GLX_ENFORCE(i == spans_.begin() || (i - 1)->end <= at, "gradients: ", what,
+              " lies in a tensor's memory");
+}
+
 // A scalar in device memory, outside the tensors.
 void GradientList::checkScalar(const void* p, int dtype, const char* what) const {
   GLX_ENFORCE(dtype == GLX_FLOAT32 || dtype == GLX_FLOAT64, "gradients: ", what,
               " is a float32 or float64");
   GLX_ENFORCE(p != nullptr && aligned(p, dtype), "gradients: ", what, " is null or misaligned");
-  const uintptr_t at = (uintptr_t)p, end = at + elementSize(dtype);
-  // spans_ is sorted and without overlap: only the last one that begins before
-  // the scalar's end can reach it
-  auto i = std::lower_bound(spans_.begin(), spans_.end(), end,
-                            [](const Span& s, uintptr_t e) { return s.at < e; });
-  GLX_ENFORCE(i == spans_.begin() || (i - 1)->end <= at, "gradients: ", what,
-              " lies in a tensor's memory");
+  checkApart(p, elementSize(dtype), what);
   deviceOf(p);
 }
 
-// The partials' memory, apart from the result.
+// The partials' memory: device memory apart from the tensors and the result.
 void GradientList::checkWorkspace(const void* p, const void* scalar) const {
   GLX_ENFORCE(p != nullptr && aligned(p, GLX_FLOAT64),
               "gradients: workspace is null or misaligned");
-  const uintptr_t w = (uintptr_t)p, end = w + (size_t)grid_ * sizeof(double);
+  const size_t bytes = (size_t)grid_ * sizeof(double);
+  const uintptr_t w = (uintptr_t)p, end = w + bytes;
   const uintptr_t q = (uintptr_t)scalar;
   GLX_ENFORCE(scalar == nullptr || q < w || q >= end,
               "gradients: a scalar lies in the workspace");
+  checkApart(p, bytes, "workspace");
+  deviceOf(p);
 }
 
 void GradientList::sum(int kind, bool root, int streamed, void* out, int outDtype,

@@ -95,6 +95,7 @@ class GradientList {
   void sum(int kind, bool root, int streamed, void* out, int outDtype, void* workspace,
            hipStream_t s) const;
 
+  void checkApart(const void* p, size_t bytes, const char* what) const;
   void checkScalar(const void* p, int dtype, const char* what) const;
   void checkWorkspace(const void* p, const void* scalar) const;
 

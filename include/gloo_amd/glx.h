@@ -686,10 +686,10 @@ int64_t glx_plan_stage(int algo, int rank, int size, int64_t count, int esize,
  * captured.  The handle is read-only after its creation, so calls on several
  * streams, or captured graphs, may run at once if each has a workspace (device
  * memory, glx_gradients_workspace_bytes, 8-byte aligned) of its own.  Short lists
- * need none: the size is 0 and the workspace may be NULL.  Scalars lie outside the
- * tensors, the workspace and each other.  Destroying
- * the handle waits for the device's work; no graph holding it may be replayed
- * afterwards.
+ * need none: the size is 0 and the workspace may be NULL.  Workspaces and scalars
+ * are device memory outside the tensors and each other; others are refused.
+ * Destroying the handle waits for the device's work; no graph holding it may be
+ * replayed afterwards.
  *
  * p is 1, 2 or INFINITY: S = sum |x|^p over all tensors (the maximum for
  * INFINITY), accumulated in float64, in an order that depends on the list

@@ -230,9 +230,83 @@ void mxOn() {
   EXPECT(m.launches.empty() && m.current == 0);
 }
 
+// A list in device 0's memory: `n` tensors of `count` floats, `stride` bytes
+// apart from `at` on; with `outs` clipped to as many others.
+struct List {
+  glx_gradients* g = nullptr;
+  std::vector<void*> grads, outs;
+  List(int n, size_t count, size_t stride, size_t at, long outsAt = -1) {
+    for (int i = 0; i < n; i++) {
+      grads.push_back(device(0, at + i * stride));
+      if (outsAt >= 0) outs.push_back(device(0, outsAt + i * stride));
+    }
+    const std::vector<size_t> counts(n, count);
+    const std::vector<int> types(n, GLX_FLOAT32);
+    g = glx_gradients_create(grads.data(), outsAt < 0 ? nullptr : outs.data(), counts.data(),
+                             types.data(), n);
+    EXPECT(g != nullptr);
+  }
+  ~List() { glx_gradients_destroy(g); }
+};
+
+// Device memory, apart from the tensors and the scalar.
+void workspace() {
+  // three tensors of 4 MiB, 8 MiB apart from 64 MiB on; outputs from 128 MiB on
+  const size_t at = 64 * kMiB, oat = 128 * kMiB, count = kMiB, step = 8 * kMiB;
+  List list(3, count, step, at, oat);
+  const size_t bytes = glx_gradients_workspace_bytes(list.g);
+  EXPECT(bytes > 0 && bytes % 8 == 0);
+  char *out = device(0, 0), *good = device(0, kMiB);
+  void* sum = device(0, 64);
+  using Call = int (*)(const List&, void* out, void* sum, void* ws);
+  const Call calls[] = {
+      [](const List& l, void* o, void*, void* w) {
+        return glx_gradients_norm(l.g, 2, o, GLX_FLOAT32, w, kStream);
+      },
+      [](const List& l, void*, void* s, void* w) {
+        return glx_gradients_power_sum(l.g, 1, s, w, kStream);
+      },
+      [](const List& l, void* o, void*, void* w) {
+        return glx_gradients_clip(l.g, 1, 2, nullptr, o, GLX_FLOAT32, w, kStream);
+      },
+      [](const List& l, void*, void*, void* w) {
+        return glx_gradients_clip(l.g, 1, 2, nullptr, nullptr, 0, w, kStream);
+      },
+  };
+  for (const Call call : calls) {
+    for (const size_t base : {at, oat}) {
+      for (const size_t i : {0, 1, 2}) {
+        char* t = device(0, base + i * step);
+        char* end = t + count * 4;
+        for (char* w : {t - bytes + 8, t, t + 4096, end - bytes, end - 8}) {
+          REFUSED(call(list, out, sum, w), "workspace lies in a tensor");
+        }
+        for (char* w : {t - bytes, end}) {
+          EXPECT(call(list, out, sum, w) == GLX_OK && m.launches.size() == 2);
+          m.launches.clear();
+        }
+      }
+    }
+    REFUSED(call(list, out, sum, pageable(0)), "not a device pointer");
+    REFUSED(call(list, out, sum, pinned(0)), "not a device pointer");
+    REFUSED(call(list, out, sum, nullptr), "workspace is null");
+    REFUSED(call(list, out, sum, good + 4), "misaligned");
+    EXPECT(call(list, out, sum, good) == GLX_OK && m.launches.size() == 2);
+    m.launches.clear();
+  }
+  REFUSED(calls[0](list, good + bytes - 8, sum, good), "in the workspace");
+  // a workspace around a whole tensor
+  List tiny(400, 16, 128, at);
+  EXPECT(glx_gradients_workspace_bytes(tiny.g) > 400 * 4);
+  REFUSED(calls[0](tiny, out, sum, device(0, at + 200 * 128 - 8)), "workspace lies in a tensor");
+  // a power sum given: no partials
+  LAUNCHED(glx_gradients_clip(list.g, 1, 2, sum, out, GLX_FLOAT32, nullptr, kStream), "clip", 0);
+}
+
 const std::map<std::string, void (*)()> kCases = {
     {"mx_pointers", mxPointers},
     {"mx_on", mxOn},
+    {"workspace", workspace},
 };
 
 }  // namespace

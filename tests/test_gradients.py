@@ -426,6 +426,24 @@ def test_scalars_apart_from_the_tensors(n):
 
 
 @gpu
+def test_workspace_apart_from_the_tensors():
+    """By the C ABI, on the host: a workspace in a gradient, or in host memory."""
+    x = torch.ones(1 << 20, device="cuda")
+    out = torch.zeros(1, device="cuda")
+    g = Gradients([x])
+    assert _lib.lib.glx_gradients_workspace_bytes(g._h) > 0
+    host = np.zeros(1 << 14)
+    for ws, message in ((x.data_ptr() + 4096, "workspace lies in a tensor"),
+                        (host.ctypes.data, "not a device pointer")):
+        for call in (lambda: _lib.lib.glx_gradients_norm(g._h, 2.0, out.data_ptr(), 5, ws, None),
+                     lambda: _lib.lib.glx_gradients_clip(g._h, 1.0, 2.0, None, None, 0, ws, None)):
+            with pytest.raises(gloo_amd.EnforceNotMet, match=message):
+                gloo_amd.errors.check(call())
+    torch.cuda.synchronize()
+    assert bool((x == 1).all()) and float(out) == 0 and not host.any()
+
+
+@gpu
 @pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
 def test_clip_of_subnormal_values(dtype):
     """Values down to the type's smallest, clipped by a norm that one large value
