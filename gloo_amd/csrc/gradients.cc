@@ -166,16 +166,24 @@ void GradientList::checkApart(const void* p, size_t bytes, const char* what) con
               " lies in a tensor's memory");
 }
 
-// A scalar in device memory, outside the tensors.
-void GradientList::checkScalar(const void* p, int dtype, const char* what) const {
+// The device of p, which is that of the tensors, if there are any.
+int GradientList::checkPlace(const void* p, const char* what) const {
+  const int device = deviceOf(p);
+  GLX_ENFORCE(nchunks_ == 0 || device == device_, "gradients: ", what,
+              " is on another device than the tensors");
+  return device;
+}
+
+// A scalar outside the tensors, on their device; returns the device.
+int GradientList::checkScalar(const void* p, int dtype, const char* what) const {
   GLX_ENFORCE(dtype == GLX_FLOAT32 || dtype == GLX_FLOAT64, "gradients: ", what,
               " is a float32 or float64");
   GLX_ENFORCE(p != nullptr && aligned(p, dtype), "gradients: ", what, " is null or misaligned");
   checkApart(p, elementSize(dtype), what);
-  deviceOf(p);
+  return checkPlace(p, what);
 }
 
-// The partials' memory: device memory apart from the tensors and the result.
+// The partials' memory: on the tensors' device, apart from them and the result.
 void GradientList::checkWorkspace(const void* p, const void* scalar) const {
   GLX_ENFORCE(p != nullptr && aligned(p, GLX_FLOAT64),
               "gradients: workspace is null or misaligned");
@@ -185,14 +193,14 @@ void GradientList::checkWorkspace(const void* p, const void* scalar) const {
   GLX_ENFORCE(scalar == nullptr || q < w || q >= end,
               "gradients: a scalar lies in the workspace");
   checkApart(p, bytes, "workspace");
-  deviceOf(p);
+  checkPlace(p, "workspace");
 }
 
 void GradientList::sum(int kind, bool root, int streamed, void* out, int outDtype,
                        void* workspace, hipStream_t s) const {
-  checkScalar(out, outDtype, "out");
+  const int device = checkScalar(out, outDtype, "out");
   if (!short_) checkWorkspace(workspace, out);
-  DeviceScope scope(device_);
+  DeviceScope scope(device);
   if (short_) {
     GLX_HIP_CHECK(
         glx::launch_short(kind, chunks_, nchunks_, false, 0, root, out, outDtype, s));
@@ -217,16 +225,20 @@ void GradientList::clip(double maxNorm, double p, const void* powerSum, void* ou
                         void* workspace, hipStream_t s) const {
   const int kind = kindOf(p);
   GLX_ENFORCE(maxNorm >= 0, "gradients: max_norm is a number >= 0, not ", maxNorm);
-  if (out != nullptr) checkScalar(out, outDtype, "norm");
+  int device = device_;
+  if (out != nullptr) device = checkScalar(out, outDtype, "norm");
   if (powerSum != nullptr) {
-    checkScalar(powerSum, GLX_FLOAT64, "power_sum");
+    const int place = checkScalar(powerSum, GLX_FLOAT64, "power_sum");
+    GLX_ENFORCE(out == nullptr || place == device,
+                "gradients: norm is on another device than power_sum");
     const uintptr_t q = (uintptr_t)powerSum, o = (uintptr_t)out;
     GLX_ENFORCE(out == nullptr || o + elementSize(outDtype) <= q || o >= q + sizeof(double),
                 "gradients: norm and power_sum share memory");
   } else if (!shortClip_) {
     checkWorkspace(workspace, out);
   }
-  DeviceScope scope(device_);
+  if (nchunks_ == 0 && out == nullptr) return;
+  DeviceScope scope(device);
   const double* part = (const double*)powerSum;
   int nparts = 1;
   if (part == nullptr) {

@@ -96,11 +96,12 @@ class GradientList {
            hipStream_t s) const;
 
   void checkApart(const void* p, size_t bytes, const char* what) const;
-  void checkScalar(const void* p, int dtype, const char* what) const;
+  int checkPlace(const void* p, const char* what) const;
+  int checkScalar(const void* p, int dtype, const char* what) const;
   void checkWorkspace(const void* p, const void* scalar) const;
 
   std::vector<Span> spans_;  // sorted
-  int device_ = 0;
+  int device_ = 0;  // of the tensors; without any, the one current at creation
   int grid_ = 1;            // workgroups of the sum, and partials
   bool short_ = false;      // one workgroup sums it all
   bool shortClip_ = false;  // and clips it

@@ -687,7 +687,8 @@ int64_t glx_plan_stage(int algo, int rank, int size, int64_t count, int esize,
  * streams, or captured graphs, may run at once if each has a workspace (device
  * memory, glx_gradients_workspace_bytes, 8-byte aligned) of its own.  Short lists
  * need none: the size is 0 and the workspace may be NULL.  Workspaces and scalars
- * are device memory outside the tensors and each other; others are refused.
+ * are memory of the tensors' device outside the tensors and each other; others are
+ * refused.  A list without elements works on the device where its scalars are.
  * Destroying the handle waits for the device's work; no graph holding it may be
  * replayed afterwards.
  *
@@ -698,7 +699,8 @@ typedef struct glx_gradients glx_gradients;
 glx_gradients* glx_gradients_create(void* const* grads, void* const* outs,
                                     const size_t* counts, const int* dtypes, int n);
 void glx_gradients_destroy(glx_gradients* g);
-/* Device index of the tensors, -1 for NULL. */
+/* Device index of the tensors (without elements: of the device that was current
+ * when the handle was made), -1 for NULL. */
 int glx_gradients_device(const glx_gradients* g);
 size_t glx_gradients_workspace_bytes(const glx_gradients* g);
 /* *sum = S, a float64 in device memory.  Ranks that hold shards of the

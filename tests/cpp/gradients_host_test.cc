@@ -303,10 +303,71 @@ void workspace() {
   LAUNCHED(glx_gradients_clip(list.g, 1, 2, sum, out, GLX_FLOAT32, nullptr, kStream), "clip", 0);
 }
 
+// Calls run where the tensors are, and scalars and workspaces are there too; a
+// list without elements runs where its result goes.
+void devices() {
+  for (const bool tensors : {false, true}) {  // no tensors at all, and empty ones
+    std::vector<void*> none(3, nullptr);
+    const std::vector<size_t> counts(3, 0);
+    const std::vector<int> types(3, GLX_BFLOAT16);
+    glx_gradients* g =
+        glx_gradients_create(none.data(), nullptr, counts.data(), types.data(), tensors ? 3 : 0);
+    EXPECT(g != nullptr && glx_gradients_workspace_bytes(g) == 0);
+    EXPECT(glx_gradients_device(g) == 0);  // the current one
+    for (int d = 0; d < kDevices; d++) {
+      void *out = device(d, 0), *sum = device(d, 64);
+      LAUNCHED(glx_gradients_norm(g, 2, out, GLX_FLOAT32, nullptr, kStream), "short", d);
+      LAUNCHED(glx_gradients_power_sum(g, 2, sum, nullptr, kStream), "short", d);
+      LAUNCHED(glx_gradients_clip(g, 1, 2, nullptr, out, GLX_FLOAT32, nullptr, kStream), "short",
+               d);
+      LAUNCHED(glx_gradients_clip(g, 1, 2, sum, out, GLX_FLOAT32, nullptr, kStream), "clip", d);
+      REFUSED(glx_gradients_clip(g, 1, 2, sum, device(1 - d, 0), GLX_FLOAT32, nullptr, kStream),
+              "another device");
+    }
+    // neither tensors nor a result: nothing to do
+    EXPECT(glx_gradients_clip(g, 1, 2, nullptr, nullptr, 0, nullptr, kStream) == GLX_OK);
+    EXPECT(glx_gradients_clip(g, 1, 2, device(1, 0), nullptr, 0, nullptr, kStream) == GLX_OK);
+    EXPECT(m.launches.empty());
+    REFUSED(glx_gradients_clip(g, -1, 2, nullptr, nullptr, 0, nullptr, kStream), "max_norm");
+    glx_gradients_destroy(g);
+  }
+  for (const size_t count : {10, 1 << 20}) {  // one workgroup, and many
+    List list(3, count, 8 * kMiB, 64 * kMiB);
+    EXPECT(glx_gradients_device(list.g) == 0);
+    void *out = device(0, 0), *sum = device(0, 64), *ws = device(0, kMiB);
+    void *far = device(1, 0), *farWs = device(1, kMiB);
+    REFUSED(glx_gradients_norm(list.g, 2, far, GLX_FLOAT32, ws, kStream), "out is on another");
+    REFUSED(glx_gradients_power_sum(list.g, 2, far, ws, kStream), "out is on another");
+    REFUSED(glx_gradients_clip(list.g, 1, 2, nullptr, far, GLX_FLOAT32, ws, kStream),
+            "norm is on another");
+    REFUSED(glx_gradients_clip(list.g, 1, 2, far, out, GLX_FLOAT32, ws, kStream),
+            "power_sum is on another");
+    if (glx_gradients_workspace_bytes(list.g) > 0) {
+      REFUSED(glx_gradients_norm(list.g, 2, out, GLX_FLOAT32, farWs, kStream),
+              "workspace is on another");
+      REFUSED(glx_gradients_clip(list.g, 1, 2, nullptr, nullptr, 0, farWs, kStream),
+              "workspace is on another");
+    }
+    m.current = 1;  // another device is current
+    EXPECT(glx_gradients_norm(list.g, 2, out, GLX_FLOAT32, ws, kStream) == GLX_OK);
+    EXPECT(glx_gradients_clip(list.g, 1, 2, sum, nullptr, 0, nullptr, kStream) == GLX_OK);
+    for (const Launch& l : m.launches) EXPECT(l.device == 0);
+    EXPECT(m.launches.size() >= 2 && m.current == 1);
+    m.launches.clear();
+    m.current = 0;
+  }
+  void* two[2] = {device(0, 0), device(1, 0)};
+  const size_t counts[2] = {4, 4};
+  const int types[2] = {GLX_FLOAT32, GLX_FLOAT32};
+  EXPECT(glx_gradients_create(two, nullptr, counts, types, 2) == nullptr &&
+         std::strstr(glx_last_error(), "tensor 1 is on another device") != nullptr);
+}
+
 const std::map<std::string, void (*)()> kCases = {
     {"mx_pointers", mxPointers},
     {"mx_on", mxOn},
     {"workspace", workspace},
+    {"devices", devices},
 };
 
 }  // namespace
