@@ -17,5 +17,9 @@ def current_stream_ptr(device):
 
 
 def as_torch_stream(stream, device):
-    """A torch.cuda.Stream, or a raw hipStream_t of `device` as one."""
-    return torch.cuda.ExternalStream(stream, device) if isinstance(stream, int) else stream
+    """A torch.cuda.Stream of `device`, or a raw hipStream_t of it as one."""
+    if isinstance(stream, int):
+        return torch.cuda.ExternalStream(stream, device)
+    if stream.device != device:
+        raise ValueError("the stream is on %s, the tensors on %s" % (stream.device, device))
+    return stream
