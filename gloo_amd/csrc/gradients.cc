@@ -151,8 +151,20 @@ GradientList::GradientList(const std::vector<void*>& grads, const std::vector<vo
   }
 }
 
+// hipFree waits for the device's work first.  It runs in the relaxed mode: a
+// capture that this thread or another one has under way, of a graph that need not
+// know the list, would be lost to it otherwise.
 GradientList::~GradientList() {
-  if (chunks_ != nullptr) (void)hipFree(chunks_);
+  if (chunks_ == nullptr) return;
+  int cur = device_;
+  (void)hipGetDevice(&cur);
+  if (cur != device_) (void)hipSetDevice(device_);
+  hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+  const bool relaxed = hipThreadExchangeStreamCaptureMode(&mode) == hipSuccess;
+  const hipError_t e = hipFree(chunks_);
+  if (relaxed) (void)hipThreadExchangeStreamCaptureMode(&mode);
+  if (cur != device_) (void)hipSetDevice(cur);
+  if (e != hipSuccess) (void)hipGetLastError();  // not the next launch's error
 }
 
 // Memory of a call outside the tensors, which other workgroups read and write.

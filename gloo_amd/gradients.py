@@ -52,7 +52,8 @@ class Gradients:
     may run at once on several streams.  The caller orders them after whatever
     wrote the gradients, and keeps the object alive while a graph holding it is
     replayed.  Make it outside of a capture, and once, not once a step: dropping
-    it waits for the device's work."""
+    it waits for the device's work (and may happen during a capture, of a graph
+    that does not hold it)."""
 
     def __init__(self, grads, outs=None):
         grads = list(grads)

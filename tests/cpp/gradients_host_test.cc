@@ -9,6 +9,7 @@
 #include <cstring>
 #include <map>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "gloo_amd/glx.h"
@@ -45,6 +46,7 @@ struct Machine {
   int current = 0, lookups = 0, frees = 0;
   size_t next = kStretch / 2;  // of hipMalloc
   hipError_t error = hipSuccess;
+  hipStreamCaptureMode mode = hipStreamCaptureModeGlobal;
   std::vector<Launch> launches;
   void (*onLaunch)(const Launch&) = nullptr;
 };
@@ -98,8 +100,15 @@ hipError_t hipMalloc(void** p, size_t n) {
   return hipSuccess;
 }
 hipError_t hipMemcpy(void*, const void*, size_t, hipMemcpyKind) { return hipSuccess; }
-hipError_t hipFree(void*) {
+hipError_t hipFree(void* p) {
   m.frees++;
+  // a capture under way in any thread makes what is not relaxed fail
+  EXPECT(m.mode == hipStreamCaptureModeRelaxed);
+  EXPECT((uintptr_t)p / kStretch == (uintptr_t)m.current + 1);  // it waits for this device
+  return hipSuccess;
+}
+hipError_t hipThreadExchangeStreamCaptureMode(hipStreamCaptureMode* mode) {
+  std::swap(m.mode, *mode);
   return hipSuccess;
 }
 void __hipRegisterFunction(void**, const void* host, char*, const char* name, unsigned, void*,
@@ -363,11 +372,25 @@ void devices() {
          std::strstr(glx_last_error(), "tensor 1 is on another device") != nullptr);
 }
 
+void destroy() {
+  glx_gradients_destroy(nullptr);
+  for (int d = 0; d < kDevices; d++) {
+    void* p = device(d, 0);
+    const size_t count = 1000;
+    const int type = GLX_FLOAT32;
+    glx_gradients* g = glx_gradients_create(&p, nullptr, &count, &type, 1);
+    EXPECT(g != nullptr && m.frees == d && m.current == 0);
+    glx_gradients_destroy(g);
+    EXPECT(m.frees == d + 1 && m.current == 0 && m.mode == hipStreamCaptureModeGlobal);
+  }
+}
+
 const std::map<std::string, void (*)()> kCases = {
     {"mx_pointers", mxPointers},
     {"mx_on", mxOn},
     {"workspace", workspace},
     {"devices", devices},
+    {"destroy", destroy},
 };
 
 }  // namespace

@@ -514,6 +514,48 @@ def test_object_dropped_while_its_work_is_queued():
 
 
 @gpu
+def test_close_waits_for_queued_work():
+    """What the handle promises: after close() nothing reads its table any more."""
+    g = Gradients([torch.ones(1 << 20, device="cuda")])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(100_000_000)
+        n = g.norm()
+    assert not s.query()
+    g.close()
+    assert s.query()
+    assert float(n) == 1024
+
+
+@gpu
+@pytest.mark.parametrize("mode", ["global", "thread_local"])
+@pytest.mark.parametrize("thread", [False, True])
+def test_dropped_while_a_graph_is_captured(mode, thread):
+    """An object that the graph does not hold, dropped by the garbage collector
+    or another thread in the middle of a capture: the capture goes on."""
+    x = torch.zeros(1 << 16, device="cuda")
+    old = Gradients([torch.ones(1 << 16, device="cuda")])
+    g = Gradients([x])
+    old.norm(), g.norm()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream(), capture_error_mode=mode):
+        x.add_(1)
+        if thread:
+            t = threading.Thread(target=old.close)
+            t.start()
+            t.join()
+        else:
+            old.close()
+        n = g.norm()
+    for step in range(1, 4):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert float(n) == 256 * step and float(g.norm()) == 256 * step
+
+
+@gpu
 def test_two_streams_at_once():
     """One handle, two streams, many calls in flight: every result is right."""
     _, views = bucket([3000017, 5], torch.float32, 3, 1)
