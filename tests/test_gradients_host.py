@@ -25,7 +25,7 @@ def program(tmp_path_factory):
     return exe
 
 
-@pytest.mark.parametrize("case", ["mx_pointers", "mx_on", "workspace", "devices", "destroy"])
+@pytest.mark.parametrize("case", ["mx_pointers", "mx_on", "workspace", "devices", "destroy", "cached"])
 def test_host(program, case):
     p = subprocess.run([program, case], capture_output=True, text=True, timeout=60)
     assert p.returncode == 0, p.stdout + p.stderr
