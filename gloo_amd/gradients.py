@@ -144,7 +144,8 @@ class Gradients:
         """Scale every gradient by min(1, max_norm / (norm + 1e-6)), in place
         or into outs, and return the norm (as norm() does): the list's own,
         or that of power_sum (a float64 on the device).  A NaN norm makes
-        every gradient NaN, an infinite one 0 (NaN where it was infinite)."""
+        every gradient NaN, an infinite one 0 (NaN where it was infinite), or
+        NaN if max_norm is infinite too (inf / inf)."""
         if stream is not None:
             with torch.cuda.stream(as_torch_stream(stream, self.device)):
                 return self.clip_norm(max_norm, p, power_sum, out)

@@ -716,8 +716,9 @@ int glx_gradients_norm(const glx_gradients* g, double p, void* norm, int norm_dt
  * is the list's own, or that of power_sum (a float64 in device memory; the
  * workspace is then not used and may be NULL), and is written to `norm` unless
  * that is NULL.  A norm of NaN makes every output NaN, an infinite one makes
- * them 0 (NaN where the gradient is infinite).  In place, tensors are not
- * touched when the coefficient is 1. */
+ * them 0 (NaN where the gradient is infinite), or NaN if max_norm is infinite
+ * too: the coefficient is inf / inf then.  In place, tensors are not touched when
+ * the coefficient is 1. */
 int glx_gradients_clip(const glx_gradients* g, double max_norm, double p,
                        const void* power_sum, void* norm, int norm_dtype, void* workspace,
                        glx_stream_t stream);

@@ -344,6 +344,27 @@ def test_clip_not_finite():
 
 
 @gpu
+@pytest.mark.parametrize("n", [5000, 1 << 20])  # one launch, and two
+@pytest.mark.parametrize("inplace", [True, False])
+@pytest.mark.parametrize("given", [False, True])
+def test_clip_of_an_infinite_norm_by_an_infinite_limit(n, inplace, given):
+    """min(1, inf / inf) is NaN; a finite norm is below the limit."""
+    x = torch.ones(n, device="cuda")
+    x[n // 2] = INF
+    y = torch.ones(9, device="cuda", dtype=torch.bfloat16)
+    outs = [x, y] if inplace else [torch.zeros_like(x), torch.zeros_like(y)]
+    g = Gradients([x, y], outs=outs)
+    s = g.power_sum() if given else None
+    assert float(g.clip_norm(INF, power_sum=s)) == INF
+    assert all(bool(torch.isnan(o).all()) for o in outs)
+    x.fill_(2)
+    y.fill_(2)
+    s = g.power_sum() if given else None
+    assert float(g.clip_norm(INF, power_sum=s)) > 2
+    assert all(bool((o == 2).all()) for o in outs)
+
+
+@gpu
 def test_clip_by_a_given_power_sum():
     _, views = bucket([1000, 70001], torch.float32, 2, 1)
     was = [v.clone() for v in views]
