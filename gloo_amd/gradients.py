@@ -122,7 +122,8 @@ class Gradients:
         """The sum of |x|^p over all gradients (the maximum of |x| for
         p = inf; p is 1, 2 or inf), accumulated in and returned as float64.
         Ranks holding shards allreduce it (SUM; MAX for inf) and give it to
-        clip_norm."""
+        clip_norm.  For p = 2, float64 values beyond about 1.3e154 make it
+        infinite, and it is 0 if all are below 1.5e-162."""
         if stream is not None:
             with torch.cuda.stream(as_torch_stream(stream, self.device)):
                 return self.power_sum(p, out)

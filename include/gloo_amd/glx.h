@@ -694,7 +694,10 @@ int64_t glx_plan_stage(int algo, int rank, int size, int64_t count, int esize,
  *
  * p is 1, 2 or INFINITY: S = sum |x|^p over all tensors (the maximum for
  * INFINITY), accumulated in float64, in an order that depends on the list
- * alone; the norm is S^(1/p).  A NaN anywhere makes both NaN. */
+ * alone; the norm is S^(1/p).  A NaN anywhere makes both NaN.  Squares of float32
+ * and shorter types neither overflow nor vanish; those of float64 values do, as
+ * float64 has it: p = 2 needs S within its range, that is values below about
+ * 1.3e154 (S is infinite above) and not all below 1.5e-162 (S is 0). */
 typedef struct glx_gradients glx_gradients;
 glx_gradients* glx_gradients_create(void* const* grads, void* const* outs,
                                     const size_t* counts, const int* dtypes, int n);
@@ -711,8 +714,11 @@ int glx_gradients_power_sum(const glx_gradients* g, double p, void* sum, void* w
 /* *norm = S^(1/p), a float32 or float64 (norm_dtype) in device memory. */
 int glx_gradients_norm(const glx_gradients* g, double p, void* norm, int norm_dtype,
                        void* workspace, glx_stream_t stream);
-/* outs[i] = grads[i] * min(1, max_norm / (norm + 1e-6)): the product in float32
- * (float64 for FLOAT64 tensors), rounded once to the tensor's type.  The norm
+/* outs[i] = grads[i] * min(1, max_norm / (norm + 1e-6)): coefficient and product
+ * rounded to float32 each (float64 for FLOAT64 tensors), the product then to the
+ * tensor's type.  A norm beyond 8.5e37 * max_norm has a coefficient that is
+ * subnormal in float32, off by up to 2^-150 (7e-5 of it where the norm is 1e41 *
+ * max_norm).  The norm
  * is the list's own, or that of power_sum (a float64 in device memory; the
  * workspace is then not used and may be NULL), and is written to `norm` unless
  * that is NULL.  A norm of NaN makes every output NaN, an infinite one makes

@@ -218,6 +218,51 @@ def test_norm_neither_overflows_nor_vanishes(value, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("n", [3, 70001])
+def test_range_of_float64_squares(n):
+    """p = 2: values whose squares leave float64's range make S infinite or 0, and
+    the clip follows; on this side of the range, and for p = 1 and inf, all is well."""
+    def grads(value):
+        return [torch.full((n,), value, device="cuda", dtype=torch.float64)]
+    big, small = grads(1.4e154), grads(1e-163)
+    g = Gradients(big)
+    assert float(g.power_sum()) == float(g.norm()) == INF
+    for p in (1.0, INF):
+        check_norm(g.norm(p), big, p)
+    assert float(g.clip_norm(1.0)) == INF and not bool(big[0].any())
+    g = Gradients(small)
+    assert float(g.power_sum()) == float(g.norm()) == 0
+    for p in (1.0, INF):
+        check_norm(g.norm(p), small, p)
+    assert float(g.clip_norm(1.0)) == 0 and bool((small[0] == 1e-163).all())
+    for value in (1.3e154 / n ** 0.5, 1e-153):  # squares and their sum are normal values
+        x = grads(value)
+        check_norm(Gradients(x).norm(), x, 2)
+    x = grads(1.3e154 / n ** 0.5)
+    was, total = x[0].clone(), exact_norm(x, 2)
+    Gradients(x).clip_norm(1.0)
+    check_clipped(x[0], was, total, 1.0, n)
+
+
+@gpu
+@pytest.mark.parametrize("n", [3, 70001])
+def test_clip_by_a_subnormal_coefficient(n):
+    """The coefficient is held in float32: below 2^-126 it is off by up to 2^-150,
+    half a step, so that the clipped value x * c is off by |x| 2^-150 beside the
+    roundings of every clip."""
+    x = torch.full((n,), 1e38, device="cuda")
+    x[1::2] = -3e37
+    was, total = x.clone(), exact_norm([x], 2)
+    for max_norm in (1e-3, 1e-6, 30.0):  # coefficients of 1e-41 and 1e-44 / sqrt(n), and more
+        out = torch.empty_like(x)
+        Gradients([x], outs=[out]).clip_norm(max_norm)
+        w = was.cpu().double().numpy()
+        exp = w * (max_norm / (total + 1e-6))
+        tol = clip_error(exp, torch.float32, n) + np.abs(w) * 2.0 ** -150
+        assert np.all(np.abs(out.cpu().double().numpy() - exp) <= tol)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=list(DTYPES))
 @pytest.mark.parametrize("p", [2.0, 1.0, INF])
 def test_norm_not_finite(dtype, p):
