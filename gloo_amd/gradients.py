@@ -103,6 +103,8 @@ class Gradients:
     def _scalar(self, t, dtype, what):
         if t.dtype != dtype or t.numel() != 1 or t.device != self.device:
             raise ValueError("%s: one %s on %s" % (what, dtype, self.device))
+        if t.is_neg():
+            raise ValueError("%s is a negated view" % what)
         return t.data_ptr()
 
     def _begin(self, dtype, out):

@@ -52,6 +52,21 @@ def cuda_tensor(dtype, n, device):
         numel=lambda: n, is_contiguous=lambda: True, is_neg=lambda: False, element_size=lambda: size)
 
 
+def test_negated_scalars_are_refused():
+    """A negated view (z.conj().imag) holds its values' opposites in memory."""
+    z = torch.zeros(1, dtype=torch.complex128).conj().imag
+    assert z.is_neg()
+    g = gloo_amd.Gradients.__new__(gloo_amd.Gradients)
+    g._h, g._ws, g._code, g.device, g.dtype = 1, 0, 6, z.device, torch.float64
+    try:
+        for call in (lambda: g.norm(out=z), lambda: g.power_sum(out=z),
+                     lambda: g.clip_norm(1.0, power_sum=z)):
+            with pytest.raises(ValueError, match="negated"):
+                call()
+    finally:
+        g._h = None  # not a handle
+
+
 def test_stream_of_another_device_is_refused(monkeypatch):
     """torch.cuda.stream() of a stream on another device leaves the tensors'
     device's current stream as it is: the call would go there unnoticed."""
