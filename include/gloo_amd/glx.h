@@ -690,7 +690,8 @@ int64_t glx_plan_stage(int algo, int rank, int size, int64_t count, int esize,
  * are memory of the tensors' device outside the tensors and each other; others are
  * refused.  A list without elements works on the device where its scalars are.
  * Destroying the handle waits for the device's work; no graph holding it may be
- * replayed afterwards.
+ * replayed afterwards.  It may be destroyed while another graph is captured, but not
+ * made.
  *
  * p is 1, 2 or INFINITY: S = sum |x|^p over all tensors (the maximum for
  * INFINITY), accumulated in float64, in an order that depends on the list
@@ -718,13 +719,12 @@ int glx_gradients_norm(const glx_gradients* g, double p, void* norm, int norm_dt
  * rounded to float32 each (float64 for FLOAT64 tensors), the product then to the
  * tensor's type.  A norm beyond 8.5e37 * max_norm has a coefficient that is
  * subnormal in float32, off by up to 2^-150 (7e-5 of it where the norm is 1e41 *
- * max_norm).  The norm
- * is the list's own, or that of power_sum (a float64 in device memory; the
- * workspace is then not used and may be NULL), and is written to `norm` unless
- * that is NULL.  A norm of NaN makes every output NaN, an infinite one makes
- * them 0 (NaN where the gradient is infinite), or NaN if max_norm is infinite
- * too: the coefficient is inf / inf then.  In place, tensors are not touched when
- * the coefficient is 1. */
+ * max_norm).  The norm is the list's own, or that of power_sum (a float64 in
+ * device memory; the workspace is then not used and may be NULL), and is written
+ * to `norm` unless that is NULL.  A norm of NaN makes every output NaN, an infinite
+ * one makes them 0 (NaN where the gradient is infinite), or NaN if max_norm is
+ * infinite too: the coefficient is inf / inf then.  In place, tensors are not
+ * touched when the coefficient is 1. */
 int glx_gradients_clip(const glx_gradients* g, double max_norm, double p,
                        const void* power_sum, void* norm, int norm_dtype, void* workspace,
                        glx_stream_t stream);

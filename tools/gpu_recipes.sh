@@ -25,6 +25,8 @@
 #   sync_control       tools/sync_control.py P = 2, 4, 8 at 4096 elements -> $O/sync_control.json
 #   ipc_probe          tools/micro/ipc_size_probe.py export / import (FLAGS, TAG) -> $O/*port.txt
 #   timeline           rank 0 of a P = 2 hop_latency run under rocprofv3 (ENGINES) -> $O/p2
+#   gradient_ops       tools/gradient_ops.py: kernel trace, FETCH_SIZE and WRITE_SIZE of the cases'
+#                      passes, whole calls, other forms -> $O/{time,fetch,write}/, $O/*.csv
 set -o pipefail
 O=${O:-gpurun_out/recipes}
 mkdir -p "$O"
@@ -118,6 +120,20 @@ recipe() {
                 --prof-name ${PROF_NAME:-hop} --copies -- tools/hop_latency.py \
                 --sizes ${SIZES:-1048576} --iters 20 ${ENGINES:+--engines $ENGINES} \
                 > "$O/p2.json" 2> "$O/p2.err" ;;
+    gradient_ops)
+      local t=tools/gradient_ops.py p="timeout -s KILL 120 rocprofv3 --output-format csv" n
+      n=norm_bf16,norm_f32_1GiB,clip_f32_256MiB,clip_mixed_large,quant_bf16_256MiB
+      n=$n,quant_f32_ef_1GiB,fold4_requant,fold8_f32_1GiB  # where bytes count
+      mkdir -p "$O/time" "$O/fetch" "$O/write"
+      timeout -k 10 200 python $t calls > "$O/calls.csv" 2> "$O/calls.err" &&
+        timeout -k 10 200 python $t forms > "$O/forms.csv" 2> "$O/forms.err" &&
+        $p --kernel-trace --stats -d "$O/time" -- python3 $t passes > "$O/time/passes.txt" \
+          2> "$O/time/err" &&
+        $p --pmc FETCH_SIZE -d "$O/fetch" -- python3 $t passes $n > "$O/fetch/passes.txt" \
+          2> "$O/fetch/err" &&
+        $p --pmc WRITE_SIZE -d "$O/write" -- python3 $t passes $n > "$O/write/passes.txt" \
+          2> "$O/write/err" &&
+        python $t summary "$O" "$O" ;;
     *) echo "unknown recipe $1" >&2; return 2 ;;
   esac
 }
