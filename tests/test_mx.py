@@ -610,6 +610,44 @@ def test_feedback_over_several_launches():
 
 # ---- with the rest of the framework ------------------------------------------
 
+def fold_of_another_process(inbox, results):
+    """A rank that folds what lies in its peer's memory."""
+    try:
+        pay, n = inbox.get(timeout=60)
+        out = torch.empty(n, device="cuda")
+        gloo_amd.errors.check(_lib.lib.glx_mx_reduce_n(
+            5, out.data_ptr(), P16(pay.data_ptr(), pay.data_ptr()), 2, n, 0.5, None))
+        torch.cuda.synchronize()
+        hop = torch.empty_like(pay)
+        gloo_amd.errors.check(_lib.lib.glx_mx_requantize_n(
+            hop.data_ptr(), P16(pay.data_ptr()), 1, n, 1.0, None))
+        torch.cuda.synchronize()
+        del pay
+        results.put((out.cpu().numpy(), hop.cpu().numpy()))
+    except BaseException as e:  # noqa: BLE001
+        results.put(repr(e))
+
+
+@gpu
+def test_payload_in_another_process():
+    """The C ABI takes memory that another process shares: kernels reach it."""
+    n = 4099
+    ctx = torch.multiprocessing.get_context("spawn")
+    inbox, results = ctx.Queue(), ctx.Queue()
+    child = ctx.Process(target=fold_of_another_process, args=(inbox, results))
+    child.start()
+    x = gradient(n, 4)
+    pay = mx.quantize(x.cuda())
+    torch.cuda.synchronize()
+    inbox.put((pay, n))
+    got = results.get(timeout=100)
+    child.join(30)
+    assert not isinstance(got, str), got
+    exp, values = payload_of(x.numpy())
+    same_bits(got[0], values.astype(np.float32))
+    assert np.array_equal(got[1][:exp.size], exp)
+
+
 @gpu
 def test_compressed_exchange_of_ranks():
     """Four thread-ranks squeeze their gradients with feedback, send the payloads
